@@ -77,7 +77,8 @@ int tq_last_error(void);                   /* sticky: cudaError of the last fail
 /* Every wait inside a kernel (the mbarrier waits of the tcgen05 GEMM, the flag wait of the
  * fused all-gather) gives up after a wall-clock limit, records a status word and lets the
  * kernel return normally; tq_sync() then turns the status into tq_last_error() = 10000 +
- * code (10021-10023: tcgen05 pipeline, 10031: a rank's gather flag never arrived). Data
+ * code (10021-10023: tcgen05 pipeline, 10031: a rank's gather flag never arrived; 10041-10043 are no
+ * waits: device arrays that describe a batch hold something impossible, see tq_kv_batch_t). Data
  * produced by a call whose wait gave up is incomplete: check tq_last_error() after
  * tq_sync() before trusting gathered outputs. The limit is two seconds unless changed here
  * (a rank can legitimately be further behind during a long prefill). tq_clear_error waits
@@ -384,6 +385,84 @@ double qwn_tc_int8_probe(int n, int iters, int accs, long long *clocks_out);
 int qwn_x_gemv_w4a8_static(const tq_qmma_weight_t *w, const float *d_x, float *d_y);
 int qwn_static_max_k(void);
 
+/* ---- operators either side of an attention layer's projections (no counterpart in the projection path of the
+ * reference): the cache that the key and value projections fill, the attention that reads it, and low-rank adapters
+ * beside any projection. Device arrays describe a batch, so a captured graph can be replayed with other lengths. */
+
+/* A paged cache: pools [pages][heads][page_size][dim] of keys and of values, bf16 (e4m3 = 0; k_scale and v_scale
+ * unused) or e4m3 (e4m3 = 1: a stored value stands for itself times the scale). dim is 64, 128 or 256; page_size
+ * any number. Pools 16-byte aligned. */
+typedef struct {
+    void *d_k, *d_v;
+    int pages, page_size, heads, dim;
+    int e4m3;
+    float k_scale, v_scale;
+} tq_kv_cache_t;
+
+/* The requests of one step. Request r has the new tokens (rows of the batch's matrices) d_start[r] ..
+ * d_start[r + 1] - 1, and d_kv_len[r] tokens in the cache INCLUDING them: its new tokens stand at the positions
+ * d_kv_len[r] - new .. d_kv_len[r] - 1. Position p lies in slot p % page_size of page d_pages[r * max_pages +
+ * p / page_size]. A request may have no new token. tokens: rows of the matrices (those from d_start[count] on are
+ * padding and left alone); max_new: no request has more new tokens (bounds what is launched). The three arrays are
+ * device memory, read when the kernels run. What is impossible in them (ranges that fall or leave the matrix,
+ * more new tokens than cached ones, more than max_pages pages, a page outside the pool) is found there: the request
+ * is skipped (a bad page's slots: not written, and read as zeros) and tq_last_error() gives 10041 after tq_sync(), or 10042 for more new tokens
+ * than max_new. */
+typedef struct {
+    int count, tokens, max_new, max_pages;
+    const int32_t *d_start;
+    const int32_t *d_kv_len;
+    const int32_t *d_pages;
+} tq_kv_batch_t;
+
+/* Rotation by position, and the norm of each query and key head before it. The first rot_dim values of a head (a
+ * multiple of 16, 0 = none) turn in pairs j: values j and j + rot_dim / 2, or 2j and 2j + 1 when interleaved, by
+ * the angle position * d_inv_freq[j] (rot_dim / 2 floats), taken in 64 bits. d_q_norm / d_k_norm (bf16[dim], NULL =
+ * none): h <- h * rsqrt(mean(h^2) + eps) * (1 + w), as x_rmsnorm_chunk. */
+typedef struct {
+    const float *d_inv_freq;
+    int rot_dim;
+    int interleaved;
+    const uint16_t *d_q_norm, *d_k_norm;
+    float eps;
+} tq_rope_t;
+
+/* Adapters of one projection [M x K]: for each of `count` adapters A [rank][K] and B [M][rank] in bf16, one after
+ * another. d_rank (NULL = all `rank`): the rank of each, at most `rank`; what lies beyond it in A and B is not
+ * used. d_scale (NULL = 1): factor of each. K % 32, M % 16 and rank % 8 are 0, rank is at most 256, count 2048. */
+typedef struct {
+    int count, rank, M, K;
+    const uint16_t *d_a, *d_b;
+    const int32_t *d_rank;
+    const float *d_scale;
+} tq_lora_t;
+
+/* Norm and rotation of the new tokens' query and key heads, then q to d_q_out (bf16 [tokens][q_heads][dim]) and k, v
+ * to the cache, rounded once. d_q, d_k, d_v: fp32 rows of the projections, ldq / ldk / ldv values apart (so they may
+ * be columns of one wide matrix); all 16-byte aligned, the strides multiples of 4. q_heads = 0 with d_q and d_q_out
+ * NULL: keys and values only. rope NULL: neither norm nor rotation. e4m3 values beyond +-448 scales become +-448.
+ * Two requests that share a page must not both write to it in one call.
+ * Returns 0, -1 (bad record), -2 (bad arguments), -3 (sizes outside the kernels' range), -4 (alignment). */
+int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq_rope_t *rope, const float *d_q,
+                    size_t ldq, int q_heads, uint16_t *d_q_out, const float *d_k, size_t ldk, const float *d_v,
+                    size_t ldv);
+/* Attention of the new tokens over each request's cache: head h of a token at position p reads key/value head
+ * h / (q_heads / heads) at positions 0..p, softmax(scale q.k) v. d_q: bf16 [tokens][q_heads][dim]. d_out: rows
+ * [tokens][ldo] of q_heads * dim values, fp32 (computed to fp32's precision throughout) or, with out_bf16, bf16
+ * (probabilities rounded to bf16 on the way). The cache behind d_kv_len[r] and unused pages are never read into a
+ * result, whatever they hold; a value that is not finite below d_kv_len[r] may reach all rows of request r.
+ * Returns as x_kv_append, and -40 when the call would have to allocate its workspace (once, on the first call: 10 MB)
+ * while the stream is being captured. */
+int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const uint16_t *d_q, int q_heads,
+                     float scale, void *d_out, size_t ldo, int out_bf16);
+/* ys[i][t] = bases[i][t] + scale (x[t] A^T) B^T with the adapter d_adapter[t] of ws[i] (negative: none, the row is
+ * bases[i][t]); up to 4 projections of one input, with the same K and number of adapters. x fp32 [T][K], bases and
+ * ys fp32 [T][M]; bases[i] may be ys[i] (added in place) or NULL, as may bases (0). Products and sums are fp32's.
+ * An adapter number beyond the pool or a rank out of range counts as none and leaves 10043 in tq_last_error(). The
+ * scratch grows with T and the ranks (-40 while the stream is being captured). Other returns as x_kv_append. */
+int qwn_x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *const *ys, int count,
+                   const float *d_x, const int32_t *d_adapter, int T);
+
 /* ---- tensor-parallel exchange: one process per GPU, NCCL loaded at run time.
  * Replaces tq_allreduce's role as the only collective (xpu/src/decode.cpp:133-154) with
  * the all-gather a column shard needs. */
@@ -545,6 +624,13 @@ void x_quantize_act_chunk_s4(const float *d_x, int K, int T, uint8_t *d_aq4, flo
                              int32_t *d_asum4);
 int x_gemm_w4a4(const tq_qmma_weight_t *w, const uint8_t *d_aq4, const float *d_as4,
                 const int32_t *d_asum4, float *d_y, int T);
+int x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq_rope_t *rope, const float *d_q,
+                size_t ldq, int q_heads, uint16_t *d_q_out, const float *d_k, size_t ldk, const float *d_v,
+                size_t ldv);
+int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const uint16_t *d_q, int q_heads, float scale,
+                 void *d_out, size_t ldo, int out_bf16 = 0);
+int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *const *ys, int count, const float *d_x,
+               const int32_t *d_adapter, int T);
 #endif /* __cplusplus */
 
 #endif /* TQ_W4A8_H */

@@ -36,7 +36,41 @@ class TqWeight(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    """tq_kv_cache_t: pools [pages][heads][page_size][dim] of keys and of values."""
+    _fields_ = [
+        ("d_k", C.c_void_p), ("d_v", C.c_void_p),
+        ("pages", C.c_int), ("page_size", C.c_int), ("heads", C.c_int), ("dim", C.c_int),
+        ("e4m3", C.c_int), ("k_scale", C.c_float), ("v_scale", C.c_float),
+    ]
+
+
+class KvBatch(C.Structure):
+    """tq_kv_batch_t: the requests of one step."""
+    _fields_ = [
+        ("count", C.c_int), ("tokens", C.c_int), ("max_new", C.c_int), ("max_pages", C.c_int),
+        ("d_start", C.c_void_p), ("d_kv_len", C.c_void_p), ("d_pages", C.c_void_p),
+    ]
+
+
+class Rope(C.Structure):
+    """tq_rope_t: rotation by position and the head norms before it."""
+    _fields_ = [
+        ("d_inv_freq", C.c_void_p), ("rot_dim", C.c_int), ("interleaved", C.c_int),
+        ("d_q_norm", C.c_void_p), ("d_k_norm", C.c_void_p), ("eps", C.c_float),
+    ]
+
+
+class Lora(C.Structure):
+    """tq_lora_t: the adapters of one projection."""
+    _fields_ = [
+        ("count", C.c_int), ("rank", C.c_int), ("M", C.c_int), ("K", C.c_int),
+        ("d_a", C.c_void_p), ("d_b", C.c_void_p), ("d_rank", C.c_void_p), ("d_scale", C.c_void_p),
+    ]
+
+
 _WP = C.POINTER(TqWeight)
+_cachep, _batchp, _ropep, _lorap = C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(Rope), C.POINTER(Lora)
 _vp, _i, _sz, _f, _d = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_double
 
 # name -> (restype, argtypes); every symbol include/tq_w4a8.h declares in its C section
@@ -133,6 +167,9 @@ SIGNATURES = {
     "qwn_x_rmsnorm_quant_chunk_pertoken": (None, [_vp, _vp, _vp, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _i]),
     "qwn_x_silu_mul_quant_chunk_pertoken": (None, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     "qwn_x_silu_mul_scatter": (_i, [_vp, _vp, _i, _i, _i, _sz, _sz]),
+    "qwn_x_kv_append": (_i, [_cachep, _batchp, _ropep, _vp, _sz, _i, _vp, _vp, _sz, _vp, _sz]),
+    "qwn_x_attn_paged": (_i, [_cachep, _batchp, _vp, _i, _f, _vp, _sz, _i]),
+    "qwn_x_lora_add": (_i, [C.POINTER(_lorap), C.POINTER(_vp), C.POINTER(_vp), _i, _vp, _vp, _i]),
     "tq_comm_rank": (_i, []), "tq_comm_world": (_i, []), "tq_comm_destroy": (None, []),
 }
 
@@ -216,6 +253,10 @@ class PackedWeight:
 def weight_array(ws):
     arr = (_WP * len(ws))(*[C.pointer(w.rec) for w in ws])
     return arr
+
+
+def lora_array(ws):
+    return (_lorap * len(ws))(*[C.pointer(w) for w in ws])
 
 
 def ptr_array(bufs):

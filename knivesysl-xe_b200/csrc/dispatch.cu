@@ -1068,6 +1068,20 @@ int qwn_x_silu_mul_scatter(const float *d_gate, const float *d_up, int T, int n,
     return x_silu_mul_scatter(d_gate, d_up, T, n, slot, col_off, ld);
 }
 
+int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq_rope_t *rope, const float *d_q,
+                    size_t ldq, int q_heads, uint16_t *d_q_out, const float *d_k, size_t ldk, const float *d_v,
+                    size_t ldv) {
+    return x_kv_append(cache, batch, rope, d_q, ldq, q_heads, d_q_out, d_k, ldk, d_v, ldv);
+}
+int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const uint16_t *d_q, int q_heads,
+                     float scale, void *d_out, size_t ldo, int out_bf16) {
+    return x_attn_paged(cache, batch, d_q, q_heads, scale, d_out, ldo, out_bf16);
+}
+int qwn_x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *const *ys, int count,
+                   const float *d_x, const int32_t *d_adapter, int T) {
+    return x_lora_add(ws, bases, ys, count, d_x, d_adapter, T);
+}
+
 int qwn_dbg_tile_dots_gemv(const tq_qmma_weight_t *w, int32_t *d_out) {
     if (!d_out) return -1;
     return tq::gemv_prepared_impl(w, nullptr, nullptr, d_out);

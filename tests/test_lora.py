@@ -1,0 +1,205 @@
+"""Low-rank adapters beside a projection (x_lora_add) against the plain 64-bit form.
+
+Tolerance: products are exact (bf16 weights, x and h in all their 24 bits), sums are fp32 with at most
+2^-24 relative to the running sum's size per step. A value of h sums K products in K/16 steps over a few
+accumulators, a value of y rank more and the base: against the sum of the absolute products that bounds a
+running sum, (K / 16 + rank + 8) 2^-24.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import attnref as ref
+
+
+def _make(pkg, count, adapters, rank, Ms, K, T, ids, ranks=True, scales=True, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    c = {"x": torch.randn(T, K, generator=g), "ids": torch.tensor(ids, dtype=torch.int32), "w": []}
+    c["x"][:, ::97] *= 20.0
+    for i in range(count):
+        w = {"a": (torch.randn(adapters, rank, K, generator=g) * K ** -0.5).to(torch.bfloat16),
+             "b": (torch.randn(adapters, Ms[i], rank, generator=g) * 0.1).to(torch.bfloat16),
+             "rank": torch.randint(0, rank + 1, (adapters,), generator=g, dtype=torch.int32) if ranks else None,
+             "scale": torch.rand(adapters, generator=g) + 0.5 if scales else None,
+             "base": torch.randn(T, Ms[i], generator=g)}
+        if ranks:                       # what lies beyond an adapter's rank must not be used
+            w["rank"][0] = rank
+            for j in range(adapters):
+                w["a"][j, int(w["rank"][j]):] = float("nan")
+                w["b"][j, :, int(w["rank"][j]):] = float("nan")
+        w["dev"] = [ref.up(w["a"]), ref.up(w["b"]), ref.up(w["rank"]) if ranks else None,
+                    ref.up(w["scale"]) if scales else None]
+        p = [d.ptr if d else None for d in w["dev"]]
+        w["rec"] = pkg.Lora(adapters, rank, Ms[i], K, *p)
+        c["w"].append(w)
+    return c
+
+
+def _run(lib, pkg, c, base="own"):
+    T = c["x"].shape[0]
+    x, ids = ref.up(c["x"]), ref.up(c["ids"])
+    if base == "inplace":
+        ys = [ref.up(w["base"]) for w in c["w"]]
+        bases = ys
+    else:
+        ys = [ref.up(torch.full_like(w["base"], 3.0)) for w in c["w"]]
+        bases = [ref.up(w["base"]) for w in c["w"]] if base == "own" else None
+    n = len(ys)
+    rc = lib.qwn_x_lora_add(pkg.lora_array([w["rec"] for w in c["w"]]), ref.ptrs(bases) if bases else None, ref.ptrs(ys),
+                            n, x.ptr, ids.ptr, T)
+    assert rc == 0
+    lib.tq_sync()
+    return [ref.down(y, torch.float32, w["base"].shape) for y, w in zip(ys, c["w"])]
+
+
+def _check(got, c, base=True):
+    K = c["x"].shape[1]
+    for y, w in zip(got, c["w"]):
+        a, b = torch.nan_to_num(w["a"].float()), torch.nan_to_num(w["b"].float())
+        bs = w["base"] if base else None
+        want = ref.lora(c["x"], c["ids"], a, b, w["rank"], w["scale"], bs)
+        size = ref.lora(c["x"].abs(), c["ids"], a.abs(), b.abs(), w["rank"], w["scale"], bs.abs() if base else None)
+        steps = K / 16 + a.shape[1] + 8
+        off = (y.double() - want).abs()
+        assert (off <= size * steps * 2.0 ** -24 + 1e-30).all(), (off / size.clamp(min=1e-30)).max() * 2.0 ** 24
+
+
+CASES = [
+    # projections' rows, adapters, rank, K, T
+    ([16], 1, 8, 32, 1),
+    ([1024], 4, 16, 5120, 1),
+    ([48, 272], 3, 24, 96, 5),
+    ([512, 64, 64], 7, 64, 1024, 33),
+    ([256], 40, 32, 512, 64),
+    ([144], 2, 256, 256, 17),
+    ([320, 320], 5, 72, 2080, 130),
+    ([1040], 3, 40, 640, 700),
+    ([64, 32, 16, 48], 300, 8, 64, 200),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
+@pytest.mark.parametrize("base", ["own", "inplace", "none"])
+def test_lora_matches_the_plain_form(lib, pkg, case, base):
+    Ms, n, rank, K, T = case
+    rng = np.random.default_rng(T + K)
+    ids = rng.integers(-1, n, T)
+    c = _make(pkg, len(Ms), n, rank, Ms, K, T, ids, seed=T)
+    _check(_run(lib, pkg, c, base), c, base != "none")
+    assert lib.tq_last_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ids", [[-1] * 40, [2] * 40, list(range(4)) * 10, [-1] * 39 + [0], [0] + [-7] * 39])
+def test_lora_orders_of_tokens(lib, pkg, ids):
+    """No adapter at all, one for all tokens, one after another, a single token with one; without rank and scale arrays."""
+    c = _make(pkg, 2, 4, 16, [96, 80], 160, 40, ids, ranks=False, scales=False, seed=3)
+    got = _run(lib, pkg, c)
+    _check(got, c)
+    for y, w in zip(got, c["w"]):       # without an adapter the base's bits come out
+        none = c["ids"] < 0
+        assert torch.equal(y[none], w["base"][none])
+
+
+@pytest.mark.gpu
+def test_lora_rows_do_not_depend_on_their_company(lib, pkg):
+    """Values that are not finite stay in their own token's row, and a token's bits do not depend on who
+    shares its tile."""
+    T = 24
+    c = _make(pkg, 1, 2, 16, [64], 128, T, [0] * T, ranks=False, seed=5)
+    clean = _run(lib, pkg, c)[0]
+    c["x"][3, 5], c["x"][9, 0] = float("nan"), float("inf")
+    got = _run(lib, pkg, c)[0]
+    keep = [t for t in range(T) if t not in (3, 9)]
+    assert torch.equal(got[keep], clean[keep])
+    assert not torch.isfinite(got[[3, 9]]).any()
+    c["ids"][:12] = -1
+    c["x"][3, 5], c["x"][9, 0] = 0.0, 0.0
+    assert torch.equal(_run(lib, pkg, c)[0][12:], clean[12:])
+
+
+@pytest.mark.gpu
+def test_lora_largest_finite_inputs(lib, pkg):
+    """x near fp32's largest value: the terms it enters the tensor core with do not overflow."""
+    c = _make(pkg, 1, 1, 8, [16], 32, 1, [0], ranks=False, scales=False, seed=6)
+    c["x"].zero_()
+    c["x"][0, 3] = 3.4028234663852886e38
+    c["w"][0]["dev"][0] = ref.up((c["w"][0]["a"].float() * 2.0 ** -40).to(torch.bfloat16))
+    c["w"][0]["a"] = (c["w"][0]["a"].float() * 2.0 ** -40).to(torch.bfloat16)
+    c["w"][0]["rec"].d_a = c["w"][0]["dev"][0].ptr
+    _check(_run(lib, pkg, c), c)
+
+
+@pytest.mark.gpu
+def test_lora_numbers_out_of_range_count_as_none(lib, pkg):
+    c = _make(pkg, 1, 3, 16, [64], 64, 6, [0, 3, 1, 99, 2, -1], seed=7, ranks=False)
+    got = _run(lib, pkg, c)[0]
+    assert lib.tq_last_error() == 10043
+    lib.tq_clear_error()
+    assert torch.equal(got[[1, 3, 5]], c["w"][0]["base"][[1, 3, 5]])
+    c["ids"][[1, 3]] = -1
+    _check([got], c)
+    c["w"][0]["rank"] = torch.tensor([16, 17, -1], dtype=torch.int32)
+    c["w"][0]["dev"][2] = ref.up(c["w"][0]["rank"])
+    c["w"][0]["rec"].d_rank = c["w"][0]["dev"][2].ptr
+    got = _run(lib, pkg, c)[0]
+    assert lib.tq_last_error() == 10043
+    lib.tq_clear_error()
+    c["w"][0]["rank"] = torch.tensor([16, 0, 0], dtype=torch.int32)
+    _check([got], c)
+
+
+@pytest.mark.gpu
+def test_lora_in_a_graph(lib, pkg):
+    c = _make(pkg, 2, 3, 16, [64, 48], 96, 9, [0, 1, 2, -1, 0, 0, 1, 2, 2], seed=8)
+    first = _run(lib, pkg, c)                       # the scratch is there now
+    x, ids = ref.up(c["x"]), ref.up(c["ids"])
+    ys, bases = ([ref.up(w["base"]) for w in c["w"]] for _ in range(2))
+    assert lib.tq_graph_capture_begin() == 0
+    rc = lib.qwn_x_lora_add(pkg.lora_array([w["rec"] for w in c["w"]]), ref.ptrs(bases), ref.ptrs(ys), 2, x.ptr, ids.ptr, 9)
+    big = lib.qwn_x_lora_add(pkg.lora_array([w["rec"] for w in c["w"]]), ref.ptrs(bases), ref.ptrs(ys), 2, x.ptr, ids.ptr,
+                             1 << 22)
+    graph = lib.tq_graph_capture_end()
+    assert rc == 0 and big == -40 and graph          # no allocation while capturing
+    lib.tq_graph_launch(graph)
+    c["ids"] = torch.tensor([1, 1, -1, 0, 2, 2, 0, 0, 1], dtype=torch.int32)
+    lib.tq_sync()
+    for y, f in zip(ys, first):
+        assert np.array_equal(ref.bits(ref.down(y, torch.float32, f.shape)), ref.bits(f))
+    v = c["ids"].numpy()
+    lib.tq_h2d(ids.ptr, v.ctypes.data, v.nbytes)
+    lib.tq_graph_launch(graph)
+    lib.tq_sync()
+    lib.tq_graph_destroy(graph)
+    _check([ref.down(y, torch.float32, f.shape) for y, f in zip(ys, first)], c)
+
+
+def test_lora_refuses_bad_arguments(pkg):
+    lib = pkg.load()
+    rec = dict(count=2, rank=16, M=64, K=64, d_a=4096, d_b=4096, d_rank=None, d_scale=None)
+    one = (C.c_void_p * 1)(4096)
+    for change, rc in [
+        (dict(count=0), -1), (dict(rank=0), -1), (dict(M=0), -1), (dict(K=0), -1), (dict(d_a=None), -1), (dict(d_b=None), -1),
+        (dict(K=48), -3), (dict(M=24), -3), (dict(rank=12), -3), (dict(rank=264), -3), (dict(count=2049), -3),
+        (dict(d_a=4104), -4), (dict(d_b=4098), -4),
+    ]:
+        ws = pkg.lora_array([pkg.Lora(**(rec | change))])
+        assert lib.qwn_x_lora_add(ws, one, one, 1, 4096, 4096, 4) == rc, change
+    ws = pkg.lora_array([pkg.Lora(**rec)])
+    assert lib.qwn_x_lora_add(None, one, one, 1, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, None, 1, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, one, 0, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, one, 5, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, one, 1, None, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, one, 1, 4096, None, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, one, 1, 4096, 4096, -1) == -2
+    assert lib.qwn_x_lora_add(ws, one, (C.c_void_p * 1)(None), 1, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, one, 1, 4100, 4096, 4) == -4
+    assert lib.qwn_x_lora_add(ws, one, (C.c_void_p * 1)(4104), 1, 4096, 4096, 4) == -4
+    two = pkg.lora_array([pkg.Lora(**rec), pkg.Lora(**(rec | dict(K=96)))])
+    pair = (C.c_void_p * 2)(4096, 4096)
+    assert lib.qwn_x_lora_add(two, pair, pair, 2, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, one, one, 1, 4096, 4096, 0) == 0
