@@ -77,7 +77,7 @@ int tq_last_error(void);                   /* sticky: cudaError of the last fail
 /* Every wait inside a kernel (the mbarrier waits of the tcgen05 GEMM, the flag wait of the
  * fused all-gather) gives up after a wall-clock limit, records a status word and lets the
  * kernel return normally; tq_sync() then turns the status into tq_last_error() = 10000 +
- * code (10021-10023: tcgen05 pipeline, 10031: a rank's gather flag never arrived; 10041-10043 are no
+ * code (10021-10024: tcgen05 pipeline, 10031: a rank's gather flag never arrived; 10041-10043 are no
  * waits: device arrays that describe a batch hold something impossible, see tq_kv_batch_t). Data
  * produced by a call whose wait gave up is incomplete: check tq_last_error() after
  * tq_sync() before trusting gathered outputs. The limit is two seconds unless changed here
@@ -451,7 +451,7 @@ int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, cons
  * [tokens][ldo] of q_heads * dim values, fp32 (computed to fp32's precision throughout) or, with out_bf16, bf16
  * (probabilities rounded to bf16 on the way). The cache behind d_kv_len[r] and unused pages are never read into a
  * result, whatever they hold; a value that is not finite below d_kv_len[r] may reach all rows of request r.
- * Returns as x_kv_append, and -40 when the call would have to allocate its workspace (once, on the first call: 10 MB)
+ * Returns as x_kv_append, and -40 when the call would have to allocate its workspace (once, on the first call: 40 MB)
  * while the stream is being captured. */
 int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const uint16_t *d_q, int q_heads,
                      float scale, void *d_out, size_t ldo, int out_bf16);

@@ -18,25 +18,12 @@
 // to [2^9, 2^10) loses only what lies 2^-34 below that). Probabilities enter the second product as
 // one bf16 term for bf16 outputs (fp16 with an e4m3 cache), and for fp32 outputs as three bf16 terms
 // or two fp16 ones, 24 and 22 bits. All sums are fp32.
-#include "kv.cuh"
+#include "attn.cuh"
 
 #include <algorithm>
 #include <math.h>
 
 namespace tq {
-
-// attn_tile.cu
-struct AttnArgs {
-    KvArgs kv;
-    const uint16_t *q;
-    void *out;
-    size_t ldo;
-    int q_heads, group;          // group = q_heads / kv heads
-    float c;                     // scale * log2(e) (times k_scale)
-    int out_bf16;
-    float *part;                 // partial tiles: [2 * CTAs][16 rows][dim + 2]
-    int *arrived;                // per CTA: parts of the tile that starts in it
-};
 
 namespace {
 
@@ -44,7 +31,6 @@ constexpr int kW = 4;                 // warps of a CTA
 constexpr int kKeys = 16;             // keys of a warp's block
 constexpr int kUnit = kW * kKeys;     // keys of a unit
 constexpr int kRows = 16;             // query rows of a tile
-constexpr int kWindow = 128;          // requests whose lengths a CTA keeps at hand
 
 template <int D, bool E4M3>
 struct Shape {
@@ -79,20 +65,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
-
-// Units of one key/value head of a request: its row tiles, each over the keys up to its last row's own.
-__device__ __forceinline__ int tile_keys(const KvRequest &q, int G, int m) {
-    const int last = min(q.n - 1, (m * kRows + kRows - 1) / G);
-    return q.total - q.n + last + 1;
-}
-__device__ __forceinline__ long long head_units(const KvRequest &q, int G) {
-    const int tiles = (q.n * G + kRows - 1) / kRows;
-    long long s = 0;
-    for (int m = 0; m < tiles; ++m) s += units_of(tile_keys(q, G, m));
-    return s;
-}
-
 template <int D, bool E4M3, bool OUT_BF16>
 __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_kernel(const AttnArgs a) {
     using S = Shape<D, E4M3>;
@@ -105,99 +77,27 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
     constexpr int kTerms = OUT_BF16 ? 1 : (E4M3 ? 2 : 3);
 
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_scan[kW];
-    __shared__ long long s_total, s_base;
-    __shared__ int s_req, s_join;
-    __shared__ KvRequest s_win[kWindow];
+    __shared__ long long s_scan[kW + 3];
+    __shared__ int s_join;
     __shared__ float s_m[kW][kRows], s_l[kW][kRows];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int G = a.group, HK = a.kv.heads;
+    const int G = a.group, cta = blockIdx.x;
     pdl_wait();
     pdl_trigger();
 
-    // ---- the whole call's units, and this CTA's stretch [u_begin, u_end) of them --------------
-    long long mine = 0;
-    for (int r = tid; r < a.kv.count; r += kW * 32) mine += head_units(kv_request(a.kv, r), G) * HK;
-    for (int off = 16; off >= 1; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
-    if (lane == 0) s_scan[warp] = mine;
-    __syncthreads();
-    if (tid == 0) {
-        long long t = 0;
-        for (int w = 0; w < kW; ++w) t += s_scan[w];
-        s_total = t;
-    }
-    __syncthreads();
-    const long long total = s_total;
-    const int ctas = (int)min((long long)gridDim.x, total);
-    const int cta = blockIdx.x;
-    if (cta >= ctas) return;
-    const long long u_begin = total * cta / ctas, u_end = total * (cta + 1) / ctas;
-
-    // ---- the request that u_begin lies in: scan blocks of requests ------------------------------
-    {
-        long long before = 0;
-        for (int r0 = 0;; r0 += kW * 32) {
-            const int r = r0 + tid;
-            const long long own = r < a.kv.count ? head_units(kv_request(a.kv, r), G) * HK : 0;
-            long long sum = own;
-            for (int off = 1; off < 32; off <<= 1) {
-                const long long o = __shfl_up_sync(0xffffffffu, sum, off);
-                if (lane >= off) sum += o;
-            }
-            __syncthreads();
-            if (lane == 31) s_scan[warp] = sum;
-            __syncthreads();
-            long long upto = before + sum, all = before;
-            for (int w = 0; w < kW; ++w) {
-                if (w < warp) upto += s_scan[w];
-                all += s_scan[w];
-            }
-            if (upto - own <= u_begin && u_begin < upto) {
-                s_req = r;
-                s_base = upto - own;
-            }
-            before = all;
-            if (all > u_begin) break;              // uniform: every thread has the same sums
-        }
-        __syncthreads();
-    }
-    int r = s_req;
-    long long at = s_base;                         // unit that request r starts at
-    int win0 = -1;
-    KvRequest req{};
-    auto fetch = [&](int rr) {                     // lengths of request rr, from the window
-        if (win0 < 0 || rr >= win0 + kWindow) {
-            __syncthreads();
-            win0 = rr;
-            const int x = rr + tid;
-            if (tid < kWindow) s_win[tid] = x < a.kv.count ? kv_request(a.kv, x) : KvRequest{0, 0, 0};
-            __syncthreads();
-        }
-        req = s_win[rr - win0];
-    };
-    fetch(r);
-    int g = 0, m = 0;
-    {
-        const long long per = head_units(req, G);
-        g = (int)((u_begin - at) / per);
-        at += per * g;
-        for (;; ++m) {
-            const int u = units_of(tile_keys(req, G, m));
-            if (at + u > u_begin) break;
-            at += u;
-        }
-    }
+    Line<kRows> line(a.kv, G, kUnit);
+    if (!line.locate<kW * 32>(s_scan, cta, gridDim.x)) return;
 
     uint8_t *const ring = smem + warp * S::kRing;
     const uint32_t ring_u = smem_u32(ring);
     const int quad = lane & 3, row_a = lane >> 2;      // this thread's tile rows: row_a and row_a + 8
 
-    for (long long u = u_begin; u < u_end;) {
-        // ---- one tile: (request r, head g, rows m * 16 ...), its units [at, at + units) ----------
-        const int keys = tile_keys(req, G, m);
-        const int units = units_of(keys);
-        const int first = (int)(u - at), last = (int)min((long long)units, u_end - at);
+    for (long long u = line.begin;;) {
+        // ---- one tile's units [first, last) ------------------------------------------------------
+        const KvRequest &req = line.q;
+        const int r = line.r, g = line.g, m = line.m, keys = line.keys, units = line.units;
+        const int first = (int)(u - line.at), last = (int)min((long long)units, line.end - line.at);
         const int rows = min(kRows, req.n * G - m * kRows);
         const int blocks = last - first;               // of this warp: one block of 16 keys per unit
 
@@ -430,7 +330,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
         __syncthreads();
         const bool whole = first == 0 && last == units;
         // a stretch's first tile goes to part 2 * cta, any later one (the last) to 2 * cta + 1
-        float *const part = a.part + (size_t)(2 * cta + (u == u_begin ? 0 : 1)) * kRows * (D + 2);
+        float *const part = a.part + (size_t)(2 * cta + (u == line.begin ? 0 : 1)) * kRows * (D + 2);
         auto store = [&](int row, int d, float4 v, float l) {
             const int rho = m * kRows + row, tok = rho / G;
             const float f = l > 0.0f ? __fdiv_rn(a.kv.v_scale, l) : 0.0f;      // no key: a row of zeros
@@ -467,12 +367,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
             }
         }
         if (!whole) {
-            // CTAs that share the tile: those whose stretches meet [at, at + units)
-            int c0 = (int)(at * ctas / total), c1 = (int)((at + units - 1) * ctas / total);
-            while (total * (c0 + 1) / ctas <= at) ++c0;
-            while (c0 > 0 && total * c0 / ctas > at) --c0;
-            while (total * (c1 + 1) / ctas <= at + units - 1) ++c1;
-            while (c1 > 0 && total * c1 / ctas > at + units - 1) --c1;
+            const int c0 = line.cta_of(line.at), c1 = line.cta_of(line.at + units - 1);    // share the tile
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -483,7 +378,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
             __syncthreads();
             if (s_join) {
                 __threadfence();
-                const int slot0 = total * c0 / ctas == at ? 2 * c0 : 2 * c0 + 1;
+                const int slot0 = line.start_of(c0) == line.at ? 2 * c0 : 2 * c0 + 1;
                 for (int x = tid; x < rows * (D / 4); x += kW * 32) {
                     const int row = x / (D / 4), d = x % (D / 4) * 4;
                     float M = -INFINITY, l = 0.0f;
@@ -505,17 +400,9 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
         }
         __syncthreads();                               // the rings are free again
 
-        // ---- the next tile
-        u = at + last;
-        if (u >= u_end) break;
-        at += units;
-        if (++m * kRows >= req.n * G) {
-            m = 0;
-            if (++g == HK) {
-                g = 0;
-                do fetch(++r); while (req.n == 0);     // one follows: u < u_end
-            }
-        }
+        u = line.at + units;
+        if (u >= line.end) break;
+        line.next();
     }
 }
 
@@ -525,13 +412,14 @@ struct AttnScratch {
 };
 AttnScratch g_attn;
 
-// The same for every call: two partial tiles of the widest head for each CTA of the largest grid.
-int attn_scratch(int ctas) {
+// The same for every call, whatever its sizes: parts of two tiles for each CTA of either kernel.
+int attn_scratch(int sms) {
     if (g_attn.part) return 0;
     if (stream_is_capturing()) return -40;
-    g_attn.part = static_cast<float *>(tq_dev_alloc((size_t)2 * ctas * kRows * (256 + 2) * sizeof(float), "attn.part"));
-    g_attn.arrived = static_cast<int *>(tq_dev_alloc((size_t)ctas * sizeof(int), "attn.arrived"));
-    TQ_CHECK(cudaMemsetAsync(g_attn.arrived, 0, (size_t)ctas * sizeof(int), stream()));
+    const size_t stream_floats = (size_t)2 * 2 * sms * kRows * (256 + 2);
+    g_attn.part = static_cast<float *>(tq_dev_alloc(std::max(stream_floats, attn_tile_part_floats(sms)) * sizeof(float), "attn.part"));
+    g_attn.arrived = static_cast<int *>(tq_dev_alloc((size_t)2 * sms * sizeof(int), "attn.arrived"));
+    TQ_CHECK(cudaMemsetAsync(g_attn.arrived, 0, (size_t)2 * sms * sizeof(int), stream()));
     return 0;
 }
 
@@ -574,7 +462,7 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     // packed rows (new tokens x group) are counted in 32 bits
     if ((long long)a.kv.tokens * q_heads > 0x7fffff00ll) return -3;
     if (!aligned16(d_q) || !aligned16(d_out) || ldo % (out_bf16 ? 8 : 4)) return -4;
-    if (const int rc = attn_scratch(2 * sm_count())) return rc;
+    if (const int rc = attn_scratch(sm_count())) return rc;
     a.kv.status = device_status_word();
     a.q = d_q;
     a.out = d_out;
@@ -585,7 +473,12 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     a.out_bf16 = out_bf16;
     a.part = g_attn.part;
     a.arrived = g_attn.arrived;
+    a.limit_ns = wait_limit_ns();
     const bool e4m3 = cache->e4m3 != 0;
+    if ((long long)a.kv.max_new * a.group > kRows) {
+        launch_attn_tile(a, e4m3, sm_count());
+        return 0;
+    }
     if (D == 64) launch_stream<64>(a, e4m3);
     else if (D == 128) launch_stream<128>(a, e4m3);
     else launch_stream<256>(a, e4m3);

@@ -57,6 +57,121 @@ __device__ __forceinline__ long long kv_row(const KvArgs &a, int r, int g, int p
     return ((long long)page * a.heads + g) * a.page_size + p % a.page_size;
 }
 
+// ---- the work of an attention call as a line of units ------------------------------------------
+// A tile is (request, kv head, ROWS packed query rows: new token x query head of the group); its
+// keys are those up to its last row's own, in units of `unit` keys. The line of all tiles' units,
+// requests outermost, is cut into equal stretches, one per CTA, whatever the lengths.
+template <int ROWS>
+struct Line {
+    const KvArgs &a;
+    const int G, unit;
+    long long total;             // units of the call
+    int ctas;                    // CTAs that have a stretch
+    long long begin, end;        // this CTA's
+    // the tile at hand
+    int r, g, m;
+    KvRequest q;
+    long long at;                // its first unit
+    int keys, units;
+
+    __device__ Line(const KvArgs &a_, int G_, int unit_) : a(a_), G(G_), unit(unit_) {}
+
+    __device__ __forceinline__ int tile_keys(const KvRequest &x, int mm) const {
+        const int last = min(x.n - 1, (int)(((long long)mm * ROWS + ROWS - 1) / G));
+        return x.total - x.n + last + 1;
+    }
+    __device__ __forceinline__ int tile_units(const KvRequest &x, int mm) const {
+        return (tile_keys(x, mm) - 1) / unit + 1;              // a tile has at least one key
+    }
+    __device__ __forceinline__ long long request_units(const KvRequest &x) const {
+        const int tiles = (x.n * G + ROWS - 1) / ROWS;
+        long long s = 0;
+        for (int mm = 0; mm < tiles; ++mm) s += tile_units(x, mm);
+        return s * a.heads;
+    }
+    // Start of CTA c's stretch, and the CTA that unit u belongs to.
+    __device__ __forceinline__ long long start_of(int c) const { return total * c / ctas; }
+    __device__ __forceinline__ int cta_of(long long u) const {
+        int c = (int)(u * ctas / total);
+        while (start_of(c + 1) <= u) ++c;
+        while (start_of(c) > u) --c;
+        return c;
+    }
+
+    // Finds this CTA's stretch and its first tile; false if it has none. All THREADS threads of the
+    // CTA call it; scan holds THREADS / 32 + 3 words of shared memory.
+    template <int THREADS>
+    __device__ bool locate(long long *scan, int cta, int grid) {
+        constexpr int W = THREADS / 32;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        long long mine = 0;
+        for (int x = tid; x < a.count; x += THREADS) mine += request_units(kv_request(a, x));
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
+        if (lane == 0) scan[warp] = mine;
+        __syncthreads();
+        total = 0;
+        for (int w = 0; w < W; ++w) total += scan[w];
+        ctas = (int)min((long long)grid, total);
+        if (cta >= ctas) return false;
+        begin = start_of(cta);
+        end = start_of(cta + 1);
+        long long before = 0;
+        for (int r0 = 0;; r0 += THREADS) {                     // blocks of requests up to the one at begin
+            const int x = r0 + tid;
+            const long long own = x < a.count ? request_units(kv_request(a, x)) : 0;
+            long long sum = own;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const long long o = __shfl_up_sync(0xffffffffu, sum, off);
+                if (lane >= off) sum += o;
+            }
+            __syncthreads();
+            if (lane == 31) scan[warp] = sum;
+            __syncthreads();
+            long long upto = before + sum, all = before;
+            for (int w = 0; w < W; ++w) {
+                if (w < warp) upto += scan[w];
+                all += scan[w];
+            }
+            if (upto - own <= begin && begin < upto) {
+                scan[W] = x;
+                scan[W + 1] = upto - own;
+            }
+            before = all;
+            if (all > begin) break;                            // the same in every thread
+        }
+        __syncthreads();
+        r = (int)scan[W];
+        at = scan[W + 1];
+        q = kv_request(a, r);
+        const long long per = request_units(q) / a.heads;
+        g = (int)((begin - at) / per);
+        at += per * g;
+        for (m = 0;; ++m) {
+            units = tile_units(q, m);
+            if (at + units > begin) break;
+            at += units;
+        }
+        keys = tile_keys(q, m);
+        return true;
+    }
+    // The tile behind this one; there is one while at + units < end.
+    __device__ __forceinline__ void next() {
+        at += units;
+        if ((long long)++m * ROWS >= (long long)q.n * G) {
+            m = 0;
+            if (++g == a.heads) {
+                g = 0;
+                do q = kv_request(a, ++r);
+                while (q.n == 0);
+            }
+        }
+        keys = tile_keys(q, m);
+        units = tile_units(q, m);
+    }
+};
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
