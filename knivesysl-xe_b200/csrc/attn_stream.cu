@@ -41,6 +41,9 @@ struct Shape {
     static constexpr int kCtas = kBlockBytes >= 16384 ? 1 : 2;
     static constexpr int kRing = kStages * kBlockBytes;
     static constexpr int kSmem = kW * kRing;
+    // What a tile costs besides its keys (first loads, the warps' and the CTAs' results joined: some 3 us
+    // of a CTA), in units at the rate that all CTAs together read the cache
+    static constexpr int kExtra = 65536 / (kW * kBlockBytes) > 1 ? 65536 / (kW * kBlockBytes) : 1;
     // the warps' results of a tile lie over the rings
     static_assert(kW * kRows * D * 4 <= kSmem, "");
 };
@@ -86,7 +89,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
     pdl_wait();
     pdl_trigger();
 
-    Line<kRows> line(a.kv, G, kUnit);
+    Line<kRows> line(a.kv, G, kUnit, S::kExtra);
     if (!line.locate<kW * 32>(s_scan, cta, gridDim.x)) return;
 
     uint8_t *const ring = smem + warp * S::kRing;
@@ -97,7 +100,8 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
         // ---- one tile's units [first, last) ------------------------------------------------------
         const KvRequest &req = line.q;
         const int r = line.r, g = line.g, m = line.m, keys = line.keys, units = line.units;
-        const int first = (int)(u - line.at), last = (int)min((long long)units, line.end - line.at);
+        const int first = line.first_unit(u), last = line.last_unit();
+        if (last <= first) break;                      // the stretch ends before the tile's first unit
         const int rows = min(kRows, req.n * G - m * kRows);
         const int blocks = last - first;               // of this warp: one block of 16 keys per unit
 
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
             }
         }
         if (!whole) {
-            const int c0 = line.cta_of(line.at), c1 = line.cta_of(line.at + units - 1);    // share the tile
+            const int c0 = line.cta_of(line.at + S::kExtra), c1 = line.cta_of(line.behind() - 1);    // share the tile
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
             __syncthreads();
             if (s_join) {
                 __threadfence();
-                const int slot0 = line.start_of(c0) == line.at ? 2 * c0 : 2 * c0 + 1;
+                const int slot0 = line.start_of(c0) >= line.at ? 2 * c0 : 2 * c0 + 1;
                 for (int x = tid; x < rows * (D / 4); x += kW * 32) {
                     const int row = x / (D / 4), d = x % (D / 4) * 4;
                     float M = -INFINITY, l = 0.0f;
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
         }
         __syncthreads();                               // the rings are free again
 
-        u = line.at + units;
+        u = line.behind();
         if (u >= line.end) break;
         line.next();
     }

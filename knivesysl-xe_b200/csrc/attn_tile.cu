@@ -25,6 +25,7 @@
 #include "tc.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tq {
 
@@ -89,6 +90,11 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&v)[32]) {
 }
 __device__ __forceinline__ void cp_async16_zero_fill(uint32_t dst, const void *src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+    return v;
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
     }
     pdl_wait();
     pdl_trigger();
-    Line<S::kRows> line(a.kv, G, kN);
+    Line<S::kRows> line(a.kv, G, kN, 2);
     const bool work = line.template locate<S::kThreads>(s_scan, cta, gridDim.x);
     if (tid == 0) joins[cta].count = 0;
     if (!work) return;
@@ -200,7 +206,8 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
         bool alive = true;
         for (long long u = line.begin; alive;) {
             const KvRequest req = line.q;
-            const int first = (int)(u - line.at), last = (int)min((long long)line.units, line.end - line.at);
+            const int first = line.first_unit(u), last = line.last_unit();
+            if (last <= first) break;
             const int end = tile_end(t, last), rows = tile_rows(t);
             const int rho = line.m * S::kRows + t * kRowsTile + row, tok = rho / G;
             const bool live = row < rows;
@@ -208,37 +215,50 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
             const int low = req.total - req.n + (line.m * S::kRows + t * kRowsTile) / G;   // seen by all rows
             float c = fabsf(a.c), m = -INFINITY, l = 0.0f;
             if (first < end) {
-                // ---- this row's queries: turned by the sign of the scale, an e4m3 cache's to fp16 times
-                // the power of two that takes the largest to [2^9, 2^10)
-                const uint4 *src = reinterpret_cast<const uint4 *>(
-                    a.q + ((size_t)(req.t0 + (live ? tok : 0)) * a.q_heads + line.g * G + (live ? rho % G : 0)) * D);
-                const uint32_t flip = a.c < 0.0f ? 0x80008000u : 0u, keep = live && a.c != 0.0f ? 0xffffffffu : 0u;
-                float upf = 1.0f;
-                if constexpr (E4M3) {
-                    uint32_t top = 0;
-                    for (int x = 0; x < D / 8; ++x) {
-                        const uint4 v = __ldg(src + x);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                // ---- the warp's 32 rows of queries, turned by the sign of the scale, whole rows per load
+                const uint32_t flip = a.c < 0.0f ? 0x80008000u : 0u, keep = a.c != 0.0f ? 0xffffffffu : 0u;
+                const long long mine = live ? ((long long)(req.t0 + tok) * a.q_heads + line.g * G + rho % G) * D : -1;
+                const uint32_t q_tile = q_smem + t * S::kQ;
+                constexpr int kQChunks = D / 8;            // 16-byte chunks of a row
+                uint4 v[8];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) top = max(top, max(w[y] << 16 & 0x7fff0000u, w[y] & 0x7fff0000u));
+                for (int x0 = 0; x0 < kQChunks; x0 += 8) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int i = (x0 + x) * 32 + lane;
+                        const long long from = __shfl_sync(0xffffffffu, mine, i / kQChunks);
+                        v[x] = from >= 0 ? __ldg(reinterpret_cast<const uint4 *>(a.q + from) + i % kQChunks) : make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int i = (x0 + x) * 32 + lane, r = (warp & 3) * 32 + i / kQChunks, ch = i % kQChunks;
+                        st_shared16(q_tile + (ch >> 3) * (kRowsTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                                    make_uint4((v[x].x ^ flip) & keep, (v[x].y ^ flip) & keep, (v[x].z ^ flip) & keep,
+                                               (v[x].w ^ flip) & keep));
+                    }
+                }
+                if constexpr (E4M3) {
+                    // own row: to fp16, times the power of two that takes its largest value to [2^9, 2^10)
+                    __syncwarp();
+                    auto place = [&](int ch) { return q_tile + (ch >> 3) * (kRowsTile * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
+                    uint32_t top = 0;
+#pragma unroll 8
+                    for (int ch = 0; ch < kQChunks; ++ch) {
+                        const uint4 w = ld_shared16(place(ch));
+                        top = max(max(top, max(w.x << 16 & 0x7fff0000u, w.x & 0x7fff0000u)), max(w.y << 16 & 0x7fff0000u, w.y & 0x7fff0000u));
+                        top = max(max(top, max(w.z << 16 & 0x7fff0000u, w.z & 0x7fff0000u)), max(w.w << 16 & 0x7fff0000u, w.w & 0x7fff0000u));
                     }
                     const int ex = min(max((int)(top >> 23) - 127, -100), 127);
-                    upf = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
+                    const float by = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
                     c *= __uint_as_float((uint32_t)(127 - 9 + ex) << 23);
-                }
-                if (a.c == 0.0f || !(c > 0.0f)) c = 1.17549435e-38f;      // scores of no size: any factor above 0
-#pragma unroll 4
-                for (int x = 0; x < D / 8; ++x) {
-                    const uint4 v = __ldg(src + x);
-                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        w[y] = (w[y] ^ flip) & keep;
-                        if constexpr (E4M3) w[y] = pack_f16(bf16_lo(w[y]) * upf, bf16_hi(w[y]) * upf);
+#pragma unroll 8
+                    for (int ch = 0; ch < kQChunks; ++ch) {
+                        const uint4 w = ld_shared16(place(ch));
+                        st_shared16(place(ch), make_uint4(pack_f16(bf16_lo(w.x) * by, bf16_hi(w.x) * by), pack_f16(bf16_lo(w.y) * by, bf16_hi(w.y) * by),
+                                                          pack_f16(bf16_lo(w.z) * by, bf16_hi(w.z) * by), pack_f16(bf16_lo(w.w) * by, bf16_hi(w.w) * by)));
                     }
-                    st_shared16(q_smem + t * S::kQ + (x >> 3) * (kRowsTile * 128) + row * 128 + (((x & 7) ^ (row & 7)) << 4),
-                                make_uint4(w[0], w[1], w[2], w[3]));
                 }
+                if (!(c > 0.0f)) c = 1.17549435e-38f;      // scores of no size: any factor above 0
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full(t));
@@ -251,27 +271,32 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                     tc_fence_after();
                     const int key0 = j * kN;
                     const bool cut = key0 + kN - 1 > low;
-                    // ---- maximum of the block
+                    // ---- maximum of the block, the next columns' load under it
                     float mx = -INFINITY;
+                    auto largest = [&](auto is_cut) {
+                        uint32_t v[2][32];
+                        tmem_ld32(s_col, v[0]);
 #pragma unroll
-                    for (int x = 0; x < kN; x += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(s_col + x, v);
-                        tmem_wait32(v);
-                        if (cut) {
-#pragma unroll
-                            for (int y = 0; y < 32; ++y)
-                                if (key0 + x + y <= limit) mx = fmaxf(mx, __uint_as_float(v[y]));
-                        } else {
+                        for (int x = 0; x < kN; x += 32) {
+                            uint32_t (&w)[32] = v[x / 32 & 1];
+                            tmem_wait32(w);
+                            if (x + 32 < kN) tmem_ld32(s_col + x + 32, v[x / 32 & 1 ^ 1]);
                             float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-                            for (int y = 0; y < 32; y += 4) {
-                                m0 = fmaxf(m0, fmaxf(__uint_as_float(v[y]), __uint_as_float(v[y + 1])));
-                                m1 = fmaxf(m1, fmaxf(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])));
+                            for (int y = 0; y < 32; y += 2) {
+                                if constexpr (decltype(is_cut)::value) {
+                                    if (key0 + x + y <= limit) m0 = fmaxf(m0, __uint_as_float(w[y]));
+                                    if (key0 + x + y + 1 <= limit) m1 = fmaxf(m1, __uint_as_float(w[y + 1]));
+                                } else {
+                                    m0 = fmaxf(m0, __uint_as_float(w[y]));
+                                    m1 = fmaxf(m1, __uint_as_float(w[y + 1]));
+                                }
                             }
                             mx = fmaxf(mx, fmaxf(m0, m1));
                         }
-                    }
+                    };
+                    if (cut) largest(std::true_type());
+                    else largest(std::false_type());
                     mx *= c;
                     const bool grows = mx > m + 8.0f;
                     if (j > first && __any_sync(0xffffffffu, grows)) {
@@ -299,37 +324,47 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                     if (grows) m = mx;
                     const float off = m == -INFINITY ? 0.0f : -m;
                     // ---- probabilities, over the scores already read
-                    float l0 = 0.0f, l1 = 0.0f;
+                    f32x2 sum = pack2(0.0f, 0.0f);
+                    const f32x2 c2 = pack2(c, c), off2 = pack2(off, off);
+                    auto weights = [&](auto is_cut) {
+                        uint32_t v[2][32];
+                        tmem_ld32(s_col, v[0]);
 #pragma unroll
-                    for (int x = 0; x < kN; x += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(s_col + x, v);
-                        tmem_wait32(v);
-                        uint32_t w[TERMS][16];
+                        for (int x = 0; x < kN; x += 32) {
+                            uint32_t (&sc)[32] = v[x / 32 & 1];
+                            tmem_wait32(sc);
+                            if (x + 32 < kN) tmem_ld32(s_col + x + 32, v[x / 32 & 1 ^ 1]);
+                            uint32_t w[TERMS][16];
 #pragma unroll
-                        for (int y = 0; y < 32; y += 2) {
-                            float p0 = exp2_approx(fmaf(__uint_as_float(v[y]), c, off));
-                            float p1 = exp2_approx(fmaf(__uint_as_float(v[y + 1]), c, off));
-                            if (cut) {
-                                if (key0 + x + y > limit) p0 = 0.0f;
-                                if (key0 + x + y + 1 > limit) p1 = 0.0f;
-                            }
-                            l0 += p0;
-                            l1 += p1;
-                            if constexpr (TERMS == 3) {
-                                split3(p0, p1, w[0][y / 2], w[1][y / 2], w[2][y / 2]);
-                            } else {
-                                w[0][y / 2] = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
-                                if constexpr (TERMS == 2) {
-                                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[0][y / 2]));
-                                    w[1][y / 2] = pack_f16(p0 - f.x, p1 - f.y);
+                            for (int y = 0; y < 32; y += 2) {
+                                float p0, p1;
+                                unpack2(fma2(pack2(__uint_as_float(sc[y]), __uint_as_float(sc[y + 1])), c2, off2), p0, p1);
+                                p0 = exp2_approx(p0);
+                                p1 = exp2_approx(p1);
+                                if constexpr (decltype(is_cut)::value) {
+                                    if (key0 + x + y > limit) p0 = 0.0f;
+                                    if (key0 + x + y + 1 > limit) p1 = 0.0f;
+                                }
+                                sum = add2(sum, pack2(p0, p1));
+                                if constexpr (TERMS == 3) {
+                                    split3(p0, p1, w[0][y / 2], w[1][y / 2], w[2][y / 2]);
+                                } else {
+                                    w[0][y / 2] = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+                                    if constexpr (TERMS == 2) {
+                                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[0][y / 2]));
+                                        w[1][y / 2] = pack_f16(p0 - f.x, p1 - f.y);
+                                    }
                                 }
                             }
+                            tmem_st16(s_col + x / 2, w[0]);
+                            if constexpr (TERMS >= 2) tmem_st16(s_col + 64 + x / 2, w[1]);
+                            if constexpr (TERMS == 3) tmem_st16(s_col + 96 + x / 2, w[2]);
                         }
-                        tmem_st16(s_col + x / 2, w[0]);
-                        if constexpr (TERMS >= 2) tmem_st16(s_col + 64 + x / 2, w[1]);
-                        if constexpr (TERMS == 3) tmem_st16(s_col + 96 + x / 2, w[2]);
-                    }
+                    };
+                    if (cut) weights(std::true_type());
+                    else weights(std::false_type());
+                    float l0, l1;
+                    unpack2(sum, l0, l1);
                     l += l0 + l1;
                     tmem_wait_st();
                     tc_fence_before();
@@ -388,20 +423,11 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                 part[(D + 1) * kRowsTile] = l;
             }
             tc_fence_before();
-            u = line.at + line.units;
-            if (u >= line.end) {
-                if (tid == 0) {
-                    // the last tile of the stretch, if it starts here and goes on: its parts
-                    JoinTile jt{req.t0, req.n, line.g, line.m, cta, cta, 0, 0};
-                    if (u > line.end && line.at >= line.begin) {
-                        jt.c1 = line.cta_of(u - 1);
-                        jt.slot0 = line.at == line.begin ? 2 * cta : 2 * cta + 1;
-                        jt.count = 1;
-                    }
-                    joins[cta] = jt;
-                }
-                break;
-            }
+            if (tid == 0 && first == 0 && last < line.units)      // the tile starts here and goes on: its parts
+                joins[cta] = JoinTile{req.t0, req.n, line.g, line.m, cta, line.cta_of(line.behind() - 1),
+                                      2 * cta + (u == line.begin ? 0 : 1), 1};
+            u = line.behind();
+            if (u >= line.end) break;
             line.next();
         }
     } else if (warp < kMmaWarp) {
@@ -431,7 +457,8 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
             return wait(bar, parity);
         };
         for (long long u = line.begin; alive;) {
-            const int first = (int)(u - line.at), last = (int)min((long long)line.units, line.end - line.at);
+            const int first = line.first_unit(u), last = line.last_unit();
+            if (last <= first) break;
             auto look_up = [&](int j) {
                 const int key = j * kN + w * kKeysW + (lane % kKeysW);
                 return j < last && key < line.keys ? kv_row(a.kv, line.r, line.g, key) : -1ll;
@@ -500,7 +527,7 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                     }
                 }
             }
-            u = line.at + line.units;
+            u = line.behind();
             if (u >= line.end) break;
             line.next();
         }
@@ -548,7 +575,8 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
             if (lead) tc_commit(empty(blk % S::kSlots));
         };
         for (long long u = line.begin; alive;) {
-            const int first = (int)(u - line.at), last = (int)min((long long)line.units, line.end - line.at);
+            const int first = line.first_unit(u), last = line.last_unit();
+            if (last <= first) break;
             int end[kT];
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
@@ -606,7 +634,7 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                 }
                 free_block(v_blk);
             }
-            u = line.at + line.units;
+            u = line.behind();
             if (u >= line.end) break;
             line.next();
         }

@@ -59,107 +59,164 @@ __device__ __forceinline__ long long kv_row(const KvArgs &a, int r, int g, int p
 
 // ---- the work of an attention call as a line of units ------------------------------------------
 // A tile is (request, kv head, ROWS packed query rows: new token x query head of the group); its
-// keys are those up to its last row's own, in units of `unit` keys. The line of all tiles' units,
+// keys are those up to its last row's own, in units of `unit` keys. On the line a tile takes `extra`
+// places, for what a tile costs besides its keys, and then one for each unit; the line of all tiles,
 // requests outermost, is cut into equal stretches, one per CTA, whatever the lengths.
 template <int ROWS>
 struct Line {
     const KvArgs &a;
-    const int G, unit;
-    long long total;             // units of the call
+    const int G, unit, extra;
+    long long total;             // places of the call
     int ctas;                    // CTAs that have a stretch
+    long long base;
+    int more;
     long long begin, end;        // this CTA's
     // the tile at hand
     int r, g, m;
     KvRequest q;
-    long long at;                // its first unit
+    long long at;                // its first place
     int keys, units;
 
-    __device__ Line(const KvArgs &a_, int G_, int unit_) : a(a_), G(G_), unit(unit_) {}
+    __device__ Line(const KvArgs &a_, int G_, int unit_, int extra_) : a(a_), G(G_), unit(unit_), extra(extra_) {}
+    // The tile's units in this CTA's stretch, [first, last), empty if the stretch ends in the extra
+    // places; `from` = the line's place that the stretch enters the tile at.
+    __device__ __forceinline__ int first_unit(long long from) const { return (int)max(from - at - extra, 0ll); }
+    __device__ __forceinline__ int last_unit() const { return (int)(min((long long)(units + extra), end - at) - extra); }
+    __device__ __forceinline__ long long behind() const { return at + extra + units; }
 
+    // A 64-bit division is some hundred instructions: 32 bits wherever the numbers have no more.
+    static __device__ __forceinline__ unsigned long long quotient(unsigned long long x, unsigned long long y) {
+        return (x | y) >> 32 ? x / y : (unsigned)x / (unsigned)y;
+    }
+    // n * G stays below 2^31 (checked by the entry point)
+    __device__ __forceinline__ int tiles_of(const KvRequest &x) const { return (int)(((unsigned)(x.n * G) + ROWS - 1) / ROWS); }
     __device__ __forceinline__ int tile_keys(const KvRequest &x, int mm) const {
-        const int last = min(x.n - 1, (int)(((long long)mm * ROWS + ROWS - 1) / G));
+        const int last = min(x.n - 1, (int)(((unsigned)mm * ROWS + ROWS - 1) / (unsigned)G));
         return x.total - x.n + last + 1;
     }
     __device__ __forceinline__ int tile_units(const KvRequest &x, int mm) const {
-        return (tile_keys(x, mm) - 1) / unit + 1;              // a tile has at least one key
+        return (int)((unsigned)(tile_keys(x, mm) - 1) / (unsigned)unit) + 1;      // a tile has at least one key
     }
-    __device__ __forceinline__ long long request_units(const KvRequest &x) const {
-        const int tiles = (x.n * G + ROWS - 1) / ROWS;
-        long long s = 0;
-        for (int mm = 0; mm < tiles; ++mm) s += tile_units(x, mm);
-        return s * a.heads;
+    // Places of one kv head of a request. A full tile mm ends at key old + floor((mm ROWS + ROWS - 1) / G), so its
+    // units are floor((old G + ROWS - 1 + ROWS mm) / (G unit)) + 1: a sum of floors of a line, by Euclid's steps.
+    __device__ long long head_places(const KvRequest &x) const {
+        const int tiles = tiles_of(x);
+        if (!tiles) return 0;
+        long long s = (long long)(extra + 1) * tiles - 1 + tile_units(x, tiles - 1);
+        unsigned long long n = tiles - 1, mod = (unsigned long long)G * unit, mul = ROWS,
+                           add = (unsigned long long)(x.total - x.n) * G + ROWS - 1;
+        while (n) {                                            // s += sum over i < n of floor((mul i + add) / mod)
+            const unsigned long long qm = quotient(mul, mod), qa = quotient(add, mod);
+            s += (long long)(n * (n - 1) / 2 * qm + n * qa);
+            mul -= qm * mod;
+            add -= qa * mod;
+            const unsigned long long top = mul * n + add;
+            n = quotient(top, mod);
+            add = top - n * mod;
+            const unsigned long long old = mod;
+            mod = mul;
+            mul = old;
+        }
+        return s;
     }
-    // Start of CTA c's stretch, and the CTA that unit u belongs to.
-    __device__ __forceinline__ long long start_of(int c) const { return total * c / ctas; }
+    // Start of CTA c's stretch (the first `more` CTAs have base + 1 units, the others base), and the
+    // CTA that place u belongs to.
+    __device__ __forceinline__ long long start_of(int c) const { return base * c + min(c, more); }
     __device__ __forceinline__ int cta_of(long long u) const {
-        int c = (int)(u * ctas / total);
-        while (start_of(c + 1) <= u) ++c;
-        while (start_of(c) > u) --c;
-        return c;
+        const long long cut = (base + 1) * more;
+        return u < cut ? (int)quotient(u, base + 1) : more + (int)quotient(u - cut, base);
     }
 
+    // Sum over the threads before this one (block-wide; scan holds THREADS / 32 words), and over all.
+    template <int THREADS>
+    static __device__ long long scan_before(long long *scan, long long own, long long &all) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        long long sum = own;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, sum, off);
+            if (lane >= off) sum += o;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = sum;
+        __syncthreads();
+        sum -= own;
+        all = 0;
+        for (int w = 0; w < THREADS / 32; ++w) {
+            const long long v = scan[w];
+            if (w < warp) sum += v;
+            all += v;
+        }
+        return sum;
+    }
     // Finds this CTA's stretch and its first tile; false if it has none. All THREADS threads of the
     // CTA call it; scan holds THREADS / 32 + 3 words of shared memory.
     template <int THREADS>
     __device__ bool locate(long long *scan, int cta, int grid) {
         constexpr int W = THREADS / 32;
-        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-        long long mine = 0;
-        for (int x = tid; x < a.count; x += THREADS) mine += request_units(kv_request(a, x));
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
-        if (lane == 0) scan[warp] = mine;
-        __syncthreads();
-        total = 0;
-        for (int w = 0; w < W; ++w) total += scan[w];
+        const int tid = threadIdx.x;
+        // the requests' places; those of the first THREADS requests stay at hand
+        const long long own0 = tid < a.count ? head_places(kv_request(a, tid)) * a.heads : 0;
+        long long mine = own0;
+        for (int x = tid + THREADS; x < a.count; x += THREADS) mine += head_places(kv_request(a, x)) * a.heads;
+        long long before = scan_before<THREADS>(scan, mine, total);
         ctas = (int)min((long long)grid, total);
         if (cta >= ctas) return false;
+        base = quotient(total, ctas);
+        more = (int)(total - base * ctas);
         begin = start_of(cta);
         end = start_of(cta + 1);
-        long long before = 0;
-        for (int r0 = 0;; r0 += THREADS) {                     // blocks of requests up to the one at begin
+        // the request that begin lies in, in blocks of THREADS
+        long long passed = 0;
+        for (int r0 = 0;; r0 += THREADS) {
             const int x = r0 + tid;
-            const long long own = x < a.count ? request_units(kv_request(a, x)) : 0;
-            long long sum = own;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const long long o = __shfl_up_sync(0xffffffffu, sum, off);
-                if (lane >= off) sum += o;
+            long long own = own0, all = total;
+            if (a.count > THREADS) {
+                own = r0 == 0 ? own0 : (x < a.count ? head_places(kv_request(a, x)) * a.heads : 0);
+                before = scan_before<THREADS>(scan, own, all);
             }
-            __syncthreads();
-            if (lane == 31) scan[warp] = sum;
-            __syncthreads();
-            long long upto = before + sum, all = before;
-            for (int w = 0; w < W; ++w) {
-                if (w < warp) upto += scan[w];
-                all += scan[w];
-            }
-            if (upto - own <= begin && begin < upto) {
+            const long long from = passed + before;
+            if (from <= begin && begin < from + own) {
                 scan[W] = x;
-                scan[W + 1] = upto - own;
+                scan[W + 1] = from;
+                scan[W + 2] = quotient(own, a.heads);
             }
-            before = all;
-            if (all > begin) break;                            // the same in every thread
+            passed += all;
+            if (passed > begin) break;                         // the same in every thread
         }
         __syncthreads();
         r = (int)scan[W];
         at = scan[W + 1];
         q = kv_request(a, r);
-        const long long per = request_units(q) / a.heads;
-        g = (int)((begin - at) / per);
+        const long long per = scan[W + 2];
+        g = (int)quotient(begin - at, per);
         at += per * g;
-        for (m = 0;; ++m) {
-            units = tile_units(q, m);
-            if (at + units > begin) break;
-            at += units;
+        // the row tile, in blocks of THREADS
+        const int tiles = tiles_of(q);
+        passed = at;
+        for (int m0 = 0;; m0 += THREADS) {
+            const int mm = m0 + tid;
+            const int own = mm < tiles ? extra + tile_units(q, mm) : 0;
+            long long all;
+            const long long from = passed + scan_before<THREADS>(scan, own, all);
+            if (from <= begin && begin < from + own) {
+                scan[W] = mm;
+                scan[W + 1] = from;
+            }
+            passed += all;
+            if (passed > begin) break;
         }
+        __syncthreads();
+        m = (int)scan[W];
+        at = scan[W + 1];
         keys = tile_keys(q, m);
+        units = tile_units(q, m);
         return true;
     }
-    // The tile behind this one; there is one while at + units < end.
+    // The tile behind this one; there is one while behind() < end.
     __device__ __forceinline__ void next() {
-        at += units;
-        if ((long long)++m * ROWS >= (long long)q.n * G) {
+        at = behind();
+        if (++m == tiles_of(q)) {
             m = 0;
             if (++g == a.heads) {
                 g = 0;
