@@ -16,6 +16,7 @@ struct AttnArgs {
     float *part;                 // partial tiles, two per CTA
     int *arrived;                // per CTA: parts of the tile that starts in it
     unsigned long long limit_ns; // of a wait (attn_tile.cu)
+    int rows, box;               // TMA copies (attn_tile.cu): rows of a pool, of a copy
 };
 
 // attn_tile.cu: tiles of 128 query rows on tcgen05

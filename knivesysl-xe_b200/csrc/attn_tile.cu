@@ -7,8 +7,9 @@
 // tensor core multiplies for one while the other's probabilities are computed. Roles:
 //   softmax  one warpgroup per tile, a thread per row: its queries into shared memory, then per block
 //            of keys S -> running maximum -> P, written over S as the next product's A operand
-//   load     four warps: the blocks of keys and values, page by page, into a ring in shared memory
-//            (cp.async; an e4m3 cache passes through registers, where it becomes fp16)
+//   load     the blocks of keys and values, page by page, into a ring in shared memory: one warp that
+//            issues TMA copies of 8 to 64 rows, or, where pages are no multiple of 8 or the cache is
+//            e4m3 (which becomes fp16 on the way), four warps through their registers
 //   mma      one warp: S = Q K^T and O += P V, and the barriers that free ring and rows
 // O is rescaled only when a row's maximum grows by more than 2^8: until then probabilities are up to
 // 2^8 instead of 1, which costs no precision, and the rescaling pass over O hardly ever runs.
@@ -24,6 +25,9 @@
 #include "attn.cuh"
 #include "tc.cuh"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -32,18 +36,24 @@ namespace tq {
 namespace {
 
 constexpr int kRowsTile = 128;
-constexpr int kLoadWarps = 4;
+// How the load warps bring a block in.
+enum Load { kTma, kRegs, kRegsE4m3 };
+constexpr int kCubic = 2;             // of four pairs of exponentials, those that the FMA pipe computes
 
-template <int D, bool E4M3, int TERMS>
+template <int D, Load LOAD, int TERMS>
 struct TileShape {
+    static constexpr int kLoadWarps = LOAD == kTma ? 1 : 4;
     static constexpr int kTiles = D <= 128 ? 2 : 1;                 // row tiles of a CTA
     static constexpr int kRows = kRowsTile * kTiles;
-    // keys of a block. More terms of P need tensor memory, dim 256 shared memory: 64 then
-    static constexpr int kKeys = TERMS == 1 && D <= 128 ? 128 : 64;
+    static constexpr int kKeys = 64;                                // of a block
+    // Score buffers of a tile. With two, the scores of block j + 1 are multiplied while the probabilities
+    // of block j are computed; more terms of P leave room for one only.
+    static constexpr int kBuf = kTiles == 1 || TERMS == 1 ? 2 : 1;
+    static constexpr int kSlotCols = 256 / (kTiles * kBuf);
     static constexpr int kBlock = kKeys * D * 2;                    // bytes of keys, or of values
-    static constexpr int kSlots = 131072 / kBlock > 8 ? 8 : 131072 / kBlock;
+    static constexpr int kRing = 131072 / kBlock > 8 ? 8 : 131072 / kBlock;
     static constexpr int kQ = kRowsTile * D * 2;                    // bytes of a tile's queries
-    static constexpr int kSmem = kTiles * kQ + kSlots * kBlock + 1024;
+    static constexpr int kSmem = kTiles * kQ + kRing * kBlock + 1024;
     static constexpr int kSoftmax = kTiles * 128;                   // threads
     static constexpr int kThreads = kSoftmax + kLoadWarps * 32 + 32;
 };
@@ -88,8 +98,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
 __device__ __forceinline__ void tmem_wait32(uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : TQ_RW8(v, 0), TQ_RW8(v, 8), TQ_RW8(v, 16), TQ_RW8(v, 24)::"memory");
 }
-__device__ __forceinline__ void cp_async16_zero_fill(uint32_t dst, const void *src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+// A box of rows of 128 bytes to shared memory, 128-byte swizzled; rows outside the tensor come as zeros.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
     uint4 v;
@@ -98,6 +111,32 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+    return d;
+}
+// 2^x for a pair, x <= 8, by the FMA pipe: x = n + f with |f| <= 1/2 (n rounded off by adding 1.5 x 2^23),
+// 2^f a cubic with the smallest relative error on that interval, 7.5e-5 (fitted by Remez exchange),
+// and n added to its exponent. x below -126 (-inf too: a masked key) gives 2^-126
+// or so, which is nothing beside the row's largest, 1.
+__device__ __forceinline__ void exp2_cubic(f32x2 x, float &e0, float &e1) {
+    float x0, x1, r0, r1;
+    unpack2(x, x0, x1);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
+    x = pack2(x0, x1);
+    const f32x2 r = add2(x, pack2(kMagicF, kMagicF));
+    const f32x2 f = add2(x, mul2(add2(r, pack2(-kMagicF, -kMagicF)), pack2(-1.0f, -1.0f)));
+    f32x2 p = fma2(pack2(0.0551716691f, 0.0551716691f), f, pack2(0.242611122f, 0.242611122f));
+    p = fma2(p, f, pack2(0.693260985f, 0.693260985f));
+    p = fma2(p, f, pack2(0.999928074f, 0.999928074f));
+    unpack2(p, e0, e1);
+    unpack2(r, r0, r1);
+    e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(r0) << 23));
+    e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(r1) << 23));
 }
 
 // A wait of this kernel, by a whole warp: bounded, and given up at once when another wait of the CTA was.
@@ -124,17 +163,21 @@ struct JoinTile {
     int count;
 };
 
-template <int D, bool E4M3, int TERMS>
-__global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn_tile_kernel(const AttnArgs a, JoinTile *joins) {
-    using S = TileShape<D, E4M3, TERMS>;
+template <int D, Load LOAD, int TERMS>
+__global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
+    attn_tile_kernel(const AttnArgs a, JoinTile *joins, const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap v_map) {
+    using S = TileShape<D, LOAD, TERMS>;
+    constexpr bool E4M3 = LOAD == kRegsE4m3;
     constexpr int kT = S::kTiles, kN = S::kKeys;
     constexpr bool OUT_BF16 = TERMS == 1;
-    constexpr uint32_t kSlotCol = 256;                 // tensor memory: O tiles, then two slots of 128 columns (S, P)
+    constexpr int kBuf = S::kBuf, kScores = kT * kBuf;
+    constexpr uint32_t kSlotCol = 256;                 // tensor memory: O tiles, then the slots of S and P
     constexpr uint32_t kQkDesc = idesc_f16(128, kN, !E4M3, false), kPvDesc = idesc_f16(128, D, !E4M3, true);
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ long long s_scan[S::kThreads / 32 + 3];
-    __shared__ __align__(8) uint64_t s_bar[2 * S::kSlots + 2 * 2 + 2 * kT + 1];
+    __shared__ __align__(8) uint64_t s_bar[2 * S::kRing + 2 * kScores + 3 * kT + 2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
 
@@ -144,37 +187,42 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
     const uint32_t q_smem = base, ring = base + kT * S::kQ;
     const uint32_t bars = smem_u32(s_bar);
     auto full = [&](int i) { return bars + 8 * i; };                        // ring slot holds a block
-    auto empty = [&](int i) { return bars + 8 * (S::kSlots + i); };         // and may be written again
-    auto s_full = [&](int i) { return bars + 8 * (2 * S::kSlots + i); };    // slot i holds scores
-    auto p_full = [&](int i) { return bars + 8 * (2 * S::kSlots + 2 + i); };
-    auto q_full = [&](int i) { return bars + 8 * (2 * S::kSlots + 4 + i); };
-    auto o_done = [&](int i) { return bars + 8 * (2 * S::kSlots + 4 + kT + i); };   // a P V product of tile i is complete
-    const uint32_t drained = bars + 8 * (2 * S::kSlots + 4 + 2 * kT);       // all products and their arrivals are done
+    auto empty = [&](int i) { return bars + 8 * (S::kRing + i); };         // and may be written again
+    auto s_full = [&](int i) { return bars + 8 * (2 * S::kRing + i); };    // slot i holds scores
+    auto p_full = [&](int i) { return bars + 8 * (2 * S::kRing + kScores + i); };
+    auto q_full = [&](int i) { return bars + 8 * (2 * S::kRing + 2 * kScores + i); };
+    auto o_done = [&](int i) { return bars + 8 * (2 * S::kRing + 2 * kScores + kT + i); };   // a P V product of tile i is complete
+    auto o_last = [&](int i) { return bars + 8 * (2 * S::kRing + 2 * kScores + 2 * kT + i); };   // the last one of a stretch's tile
+    const uint32_t drained = bars + 8 * (2 * S::kRing + 2 * kScores + 3 * kT);       // all products and their arrivals are done
+
+    const uint32_t landed = drained + 8;               // a block that the load warp has to complete itself
 
     if (tid == 0) {
         mbar_init(drained, 1);
-        for (int i = 0; i < S::kSlots; ++i) {
-            mbar_init(full(i), kLoadWarps);
+        mbar_init(landed, 1);
+        for (int i = 0; i < S::kRing; ++i) {
+            mbar_init(full(i), S::kLoadWarps);
             mbar_init(empty(i), 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kScores; ++i) {
             mbar_init(s_full(i), 1);
             mbar_init(p_full(i), 4);
         }
         for (int i = 0; i < kT; ++i) {
             mbar_init(q_full(i), 4);
             mbar_init(o_done(i), 1);
+            mbar_init(o_last(i), 1);
         }
         mbar_init_fence();
         s_gave_up = 0;
     }
     pdl_wait();
     pdl_trigger();
-    Line<S::kRows> line(a.kv, G, kN, 2);
+    Line<S::kRows> line(a.kv, G, kN, 4);
     const bool work = line.template locate<S::kThreads>(s_scan, cta, gridDim.x);
     if (tid == 0) joins[cta].count = 0;
     if (!work) return;
-    constexpr int kMmaWarp = S::kSoftmax / 32 + kLoadWarps;
+    constexpr int kMmaWarp = S::kSoftmax / 32 + S::kLoadWarps;
     if (warp == kMmaWarp) {
         tmem_alloc(smem_u32(&s_tmem), 512);
         tmem_relinquish();
@@ -202,7 +250,7 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lane_col = tmem + ((uint32_t)(warp & 3) << 21);
         const uint32_t o_col = lane_col + t * D;
-        uint32_t s_phase = 0, o_count = 0;               // a bit per slot; products of this tile
+        uint32_t s_phase = 0, o_count = 0, tiles_done = 0;   // a bit per slot; products of this tile; tiles
         bool alive = true;
         for (long long u = line.begin; alive;) {
             const KvRequest req = line.q;
@@ -264,43 +312,38 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                 if (lane == 0) mbar_arrive(q_full(t));
 
                 for (int j = first; j < end; ++j) {
-                    const int slot = kT == 2 ? t : (j - first) & 1;
-                    const uint32_t s_col = lane_col + kSlotCol + slot * 128;
+                    const int slot = t * kBuf + (kBuf == 2 ? (j - first) & 1 : 0);
+                    const uint32_t s_col = lane_col + kSlotCol + slot * S::kSlotCols;
                     if (!wait(s_full(slot), s_phase >> slot & 1)) { alive = false; break; }
                     s_phase ^= 1u << slot;
                     tc_fence_after();
                     const int key0 = j * kN;
                     const bool cut = key0 + kN - 1 > low;
-                    // ---- maximum of the block, the next columns' load under it
-                    float mx = -INFINITY;
-                    auto largest = [&](auto is_cut) {
-                        uint32_t v[2][32];
-                        tmem_ld32(s_col, v[0]);
+                    // ---- maximum of the block
+                    uint32_t v0[32], v1[32];
+                    tmem_ld32(s_col, v0);
+                    tmem_ld32(s_col + 32, v1);
+                    tmem_wait32(v0);
+                    tmem_wait32(v1);
+                    if (cut) {
 #pragma unroll
-                        for (int x = 0; x < kN; x += 32) {
-                            uint32_t (&w)[32] = v[x / 32 & 1];
-                            tmem_wait32(w);
-                            if (x + 32 < kN) tmem_ld32(s_col + x + 32, v[x / 32 & 1 ^ 1]);
-                            float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-                            for (int y = 0; y < 32; y += 2) {
-                                if constexpr (decltype(is_cut)::value) {
-                                    if (key0 + x + y <= limit) m0 = fmaxf(m0, __uint_as_float(w[y]));
-                                    if (key0 + x + y + 1 <= limit) m1 = fmaxf(m1, __uint_as_float(w[y + 1]));
-                                } else {
-                                    m0 = fmaxf(m0, __uint_as_float(w[y]));
-                                    m1 = fmaxf(m1, __uint_as_float(w[y + 1]));
-                                }
-                            }
-                            mx = fmaxf(mx, fmaxf(m0, m1));
+                        for (int y = 0; y < 32; ++y) {
+                            if (key0 + y > limit) v0[y] = 0xff800000u;
+                            if (key0 + 32 + y > limit) v1[y] = 0xff800000u;
                         }
-                    };
-                    if (cut) largest(std::true_type());
-                    else largest(std::false_type());
+                    }
+                    float mx = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                    for (int y = 0; y < 32; y += 2) {
+                        mx = max3(mx, __uint_as_float(v0[y]), __uint_as_float(v0[y + 1]));
+                        mx1 = max3(mx1, __uint_as_float(v1[y]), __uint_as_float(v1[y + 1]));
+                    }
+                    mx = fmaxf(mx, mx1);
                     mx *= c;
                     const bool grows = mx > m + 8.0f;
                     if (j > first && __any_sync(0xffffffffu, grows)) {
-                        // the product of block j - 1 must be in O
+                        // The product of block j - 1 must be in O. That of j - 2 is (the scores of block j were
+                        // multiplied behind it), so the barrier is at most one phase behind.
                         if (!wait(o_done(t), (o_count - 1) & 1)) { alive = false; break; }
                         tc_fence_after();
                         const float f = grows ? exp2_approx(m - mx) : 1.0f;
@@ -323,46 +366,39 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                     }
                     if (grows) m = mx;
                     const float off = m == -INFINITY ? 0.0f : -m;
-                    // ---- probabilities, over the scores already read
+                    // ---- probabilities, over the scores
                     f32x2 sum = pack2(0.0f, 0.0f);
                     const f32x2 c2 = pack2(c, c), off2 = pack2(off, off);
-                    auto weights = [&](auto is_cut) {
-                        uint32_t v[2][32];
-                        tmem_ld32(s_col, v[0]);
+                    auto weights = [&](const uint32_t (&sc)[32], int x) {
+                        uint32_t w[TERMS][16];
 #pragma unroll
-                        for (int x = 0; x < kN; x += 32) {
-                            uint32_t (&sc)[32] = v[x / 32 & 1];
-                            tmem_wait32(sc);
-                            if (x + 32 < kN) tmem_ld32(s_col + x + 32, v[x / 32 & 1 ^ 1]);
-                            uint32_t w[TERMS][16];
-#pragma unroll
-                            for (int y = 0; y < 32; y += 2) {
-                                float p0, p1;
-                                unpack2(fma2(pack2(__uint_as_float(sc[y]), __uint_as_float(sc[y + 1])), c2, off2), p0, p1);
+                        for (int y = 0; y < 32; y += 2) {
+                            float p0, p1;
+                            const f32x2 z = fma2(pack2(__uint_as_float(sc[y]), __uint_as_float(sc[y + 1])), c2, off2);
+                            if (TERMS == 1 && (y & 7) >= 8 - 2 * kCubic) {
+                                exp2_cubic(z, p0, p1);
+                            } else {
+                                unpack2(z, p0, p1);
                                 p0 = exp2_approx(p0);
                                 p1 = exp2_approx(p1);
-                                if constexpr (decltype(is_cut)::value) {
-                                    if (key0 + x + y > limit) p0 = 0.0f;
-                                    if (key0 + x + y + 1 > limit) p1 = 0.0f;
-                                }
-                                sum = add2(sum, pack2(p0, p1));
-                                if constexpr (TERMS == 3) {
-                                    split3(p0, p1, w[0][y / 2], w[1][y / 2], w[2][y / 2]);
-                                } else {
-                                    w[0][y / 2] = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
-                                    if constexpr (TERMS == 2) {
-                                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[0][y / 2]));
-                                        w[1][y / 2] = pack_f16(p0 - f.x, p1 - f.y);
-                                    }
+                            }
+                            sum = add2(sum, pack2(p0, p1));
+                            if constexpr (TERMS == 3) {
+                                split3(p0, p1, w[0][y / 2], w[1][y / 2], w[2][y / 2]);
+                            } else {
+                                w[0][y / 2] = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+                                if constexpr (TERMS == 2) {
+                                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[0][y / 2]));
+                                    w[1][y / 2] = pack_f16(p0 - f.x, p1 - f.y);
                                 }
                             }
-                            tmem_st16(s_col + x / 2, w[0]);
-                            if constexpr (TERMS >= 2) tmem_st16(s_col + 64 + x / 2, w[1]);
-                            if constexpr (TERMS == 3) tmem_st16(s_col + 96 + x / 2, w[2]);
                         }
+                        tmem_st16(s_col + x / 2, w[0]);
+                        if constexpr (TERMS >= 2) tmem_st16(s_col + 64 + x / 2, w[1]);
+                        if constexpr (TERMS == 3) tmem_st16(s_col + 96 + x / 2, w[2]);
                     };
-                    if (cut) weights(std::true_type());
-                    else weights(std::false_type());
+                    weights(v0, 0);
+                    weights(v1, 32);
                     float l0, l1;
                     unpack2(sum, l0, l1);
                     l += l0 + l1;
@@ -372,7 +408,7 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                     if (lane == 0) mbar_arrive(p_full(slot));
                     ++o_count;
                 }
-                if (!alive || !wait(o_done(t), (o_count - 1) & 1)) break;
+                if (!alive || !wait(o_last(t), tiles_done++ & 1)) break;
                 tc_fence_after();
             }
             // ---- the tile's rows, or this CTA's part of them
@@ -432,147 +468,173 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
         }
     } else if (warp < kMmaWarp) {
         // ================================ load ===================================================
-        constexpr int kKeysW = kN / kLoadWarps;            // keys of a warp
-        constexpr int kChunks = (E4M3 ? D : 2 * D) / 16;   // of a cached row
-        constexpr int kLoads = kKeysW * kChunks / 32;
-        const int w = warp - S::kSoftmax / 32;
-        int at = 0;                                        // blocks so far; slot at % kSlots
-        int told = 0;                                      // of them, handed over
+        int at = 0;                                        // blocks so far; slot at % kRing
         bool alive = true;
-        auto hand_over = [&](int upto) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            for (; told < upto; ++told)
-                if (lane == 0) mbar_arrive(full(told % S::kSlots));
-        };
         auto wait_empty = [&]() {
-            if (at < S::kSlots) return true;
-            const uint32_t bar = empty(at % S::kSlots), parity = ((at / S::kSlots) - 1) & 1;
-            if constexpr (!E4M3) {
-                if (!mbar_test_wait_warp(bar, parity)) {   // before a wait, what has been started is finished and handed over
-                    cp_async_wait<0>();
-                    hand_over(at);
-                }
-            }
-            return wait(bar, parity);
+            return at < S::kRing || wait(empty(at % S::kRing), ((at / S::kRing) - 1) & 1);
         };
-        for (long long u = line.begin; alive;) {
-            const int first = line.first_unit(u), last = line.last_unit();
-            if (last <= first) break;
-            auto look_up = [&](int j) {
-                const int key = j * kN + w * kKeysW + (lane % kKeysW);
-                return j < last && key < line.keys ? kv_row(a.kv, line.r, line.g, key) : -1ll;
-            };
-            long long row = look_up(first);
-            if constexpr (E4M3) {
-                uint4 held[kLoads];
-                auto load = [&](const uint8_t *pool) {
-#pragma unroll
-                    for (int i = 0; i < kLoads; ++i) {
-                        const int x = i * 32 + lane;
-                        const long long r = __shfl_sync(0xffffffffu, row, x / kChunks);
-                        held[i] = r >= 0 ? __ldg(reinterpret_cast<const uint4 *>(pool + (size_t)r * D + (x % kChunks) * 16))
-                                         : make_uint4(0, 0, 0, 0);
-                    }
+        if constexpr (LOAD == kTma) {
+            uint32_t landings = 0;
+            for (long long u = line.begin; alive;) {
+                const int first = line.first_unit(u), last = line.last_unit();
+                if (last <= first) break;
+                const int box = a.box, boxes = kN / box;
+                // a lane per box: its first row in the pools; behind the last page's rows (read as zeros) for a bad page
+                auto look_up = [&](int j) {
+                    const int key = j * kN + lane * box;
+                    if (j >= last || lane >= boxes || key >= line.keys) return a.rows;
+                    const long long row = kv_row(a.kv, line.r, line.g, key);
+                    return row < 0 ? a.rows : (int)row;
                 };
-                auto store = [&]() {                       // chunk of 16 values -> two of 8 fp16 values
-                    const uint32_t dst = ring + (at % S::kSlots) * S::kBlock;
-#pragma unroll
-                    for (int i = 0; i < kLoads; ++i) {
-                        const int x = i * 32 + lane, key = w * kKeysW + x / kChunks, ch = x % kChunks * 2;
-                        const uint32_t to = dst + (ch >> 3) * (kN * 128) + key * 128;
-                        const uint32_t v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
-                        uint32_t f[8];
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            f[2 * y] = e4m3_to_f16((uint16_t)v[y]);
-                            f[2 * y + 1] = e4m3_to_f16((uint16_t)(v[y] >> 16));
-                        }
-                        st_shared16(to + (((ch & 7) ^ (key & 7)) << 4), make_uint4(f[0], f[1], f[2], f[3]));
-                        st_shared16(to + ((((ch & 7) + 1) ^ (key & 7)) << 4), make_uint4(f[4], f[5], f[6], f[7]));
-                    }
-                };
-                load(a.kv.k);
-                for (int j = first; j < last; ++j) {
-                    if (!wait_empty()) { alive = false; break; }
-                    store();
-                    hand_over(++at);
-                    load(a.kv.v);
-                    row = look_up(j + 1);
-                    if (!wait_empty()) { alive = false; break; }
-                    store();
-                    hand_over(++at);
-                    load(a.kv.k);
-                }
-            } else {
+                int next = look_up(first);
                 for (int j = first; j < last && alive; ++j) {
-                    const long long mine = row;
-                    row = look_up(j + 1);
+                    const int row = next;
+                    next = look_up(j + 1);
+                    const int rest = line.keys - j * kN;       // rows behind the request's last key: whatever the page holds
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
                         if (!wait_empty()) { alive = false; break; }
-                        const uint32_t dst = ring + (at % S::kSlots) * S::kBlock;
-                        const uint8_t *pool = kv ? a.kv.v : a.kv.k;
+                        const uint32_t dst = ring + (at % S::kRing) * S::kBlock;
+                        const bool tail = kv && rest < kN;     // a probability of 0 times that must be 0: zeros instead
+                        const uint32_t bar = tail ? landed : full(at % S::kRing);
+                        if (lane == 0) mbar_expect_tx(bar, S::kBlock);
+                        __syncwarp();
+                        if (lane < boxes)
 #pragma unroll
-                        for (int i = 0; i < kLoads; ++i) {
-                            const int x = i * 32 + lane, key = w * kKeysW + x / kChunks, ch = x % kChunks;
-                            const long long r = __shfl_sync(0xffffffffu, mine, x / kChunks);
-                            cp_async16_zero_fill(dst + (ch >> 3) * (kN * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4),
-                                                 pool + (size_t)(r < 0 ? 0 : r) * (2 * D) + ch * 16, r >= 0);
+                            for (int x = 0; x < D / 64; ++x)
+                                tma_load(dst + x * (kN * 128) + lane * box * 128, kv ? &v_map : &k_map, x * 64, row, bar);
+                        if (tail) {
+                            if (!wait(landed, landings++ & 1)) { alive = false; break; }
+                            for (int i = lane; i < (kN - rest) * (D / 8); i += 32)
+                                st_shared16(dst + (i & 7) * 16 + (i >> 3) % (D / 64) * (kN * 128) + (rest + (i >> 3) / (D / 64)) * 128,
+                                            make_uint4(0, 0, 0, 0));
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(full(at % S::kRing));
                         }
-                        cp_async_commit();
                         ++at;
-                        cp_async_wait<2>();
-                        if (at - 2 > told) hand_over(at - 2);
                     }
                 }
+                u = line.behind();
+                if (u >= line.end) break;
+                line.next();
             }
-            u = line.behind();
-            if (u >= line.end) break;
-            line.next();
+            // the copies in flight end before the CTA does: the products wait for them, unless a wait gave up
+            if (!alive)
+                for (int i = max(0, at - S::kRing); i < at; ++i)
+                    mbar_wait_bounded(full(i % S::kRing), (i / S::kRing) & 1, a.kv.status, 24, a.limit_ns);
+            __syncwarp();
+        } else {
+            constexpr int kKeysW = kN / S::kLoadWarps;         // keys of a warp
+            constexpr int kChunks = (E4M3 ? D : 2 * D) / 16;   // of a cached row
+            constexpr int kAll = kKeysW * kChunks / 32, kLoads = kAll > 8 ? 8 : kAll;      // loads of a block, in one go
+            const int w = warp - S::kSoftmax / 32;
+            for (long long u = line.begin; alive;) {
+                const int first = line.first_unit(u), last = line.last_unit();
+                if (last <= first) break;
+                auto look_up = [&](int j) {
+                    const int key = j * kN + w * kKeysW + (lane % kKeysW);
+                    return j < last && key < line.keys ? kv_row(a.kv, line.r, line.g, key) : -1ll;
+                };
+                long long row = look_up(first);
+                uint4 held[kLoads];
+                auto load = [&](const uint8_t *pool, int part) {
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        const int x = (part * kLoads + i) * 32 + lane;
+                        const long long r = __shfl_sync(0xffffffffu, row, x / kChunks);
+                        held[i] = r >= 0 ? __ldg(reinterpret_cast<const uint4 *>(pool + ((size_t)r * kChunks + x % kChunks) * 16))
+                                         : make_uint4(0, 0, 0, 0);
+                    }
+                };
+                auto store = [&](int part) {
+                    const uint32_t dst = ring + (at % S::kRing) * S::kBlock;
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        const int x = (part * kLoads + i) * 32 + lane, key = w * kKeysW + x / kChunks;
+                        if constexpr (E4M3) {              // 16 values -> two chunks of 8 fp16 values
+                            const int ch = x % kChunks * 2;
+                            const uint32_t to = dst + (ch >> 3) * (kN * 128) + key * 128;
+                            const uint32_t v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+                            uint32_t f[8];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                f[2 * y] = e4m3_to_f16((uint16_t)v[y]);
+                                f[2 * y + 1] = e4m3_to_f16((uint16_t)(v[y] >> 16));
+                            }
+                            st_shared16(to + (((ch & 7) ^ (key & 7)) << 4), make_uint4(f[0], f[1], f[2], f[3]));
+                            st_shared16(to + ((((ch & 7) + 1) ^ (key & 7)) << 4), make_uint4(f[4], f[5], f[6], f[7]));
+                        } else {
+                            const int ch = x % kChunks;
+                            st_shared16(dst + (ch >> 3) * (kN * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4), held[i]);
+                        }
+                    }
+                };
+                // the next block's first loads are under way while this one waits for its slot
+                load(a.kv.k, 0);
+                for (int j = first; j < last && alive; ++j) {
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        if (!wait_empty()) { alive = false; break; }
+                        store(0);
+#pragma unroll
+                        for (int part = 1; part < kAll / kLoads; ++part) {
+                            load(kv ? a.kv.v : a.kv.k, part);
+                            store(part);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(full(at % S::kRing));
+                        ++at;
+                        if (kv) row = look_up(j + 1);
+                        load(kv ? a.kv.k : a.kv.v, 0);
+                    }
+                }
+                u = line.behind();
+                if (u >= line.end) break;
+                line.next();
+            }
         }
-        cp_async_wait<0>();
-        hand_over(at);
     } else {
         // ================================ mma ====================================================
         uint32_t p_phase = 0, q_phase = 0;                 // a bit per slot, per tile
         int at = 0;                                        // ring blocks so far (keys and values alternate)
         const bool lead = elect_one();
         auto score = [&](int t, int slot, int blk) {       // S = Q K^T
-            const uint32_t k_smem = ring + (blk % S::kSlots) * S::kBlock;
+            const uint32_t k_smem = ring + (blk % S::kRing) * S::kBlock;
             if (lead) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_f16_ss(tmem + kSlotCol + slot * 128,
+                    mma_f16_ss(tmem + kSlotCol + slot * S::kSlotCols,
                                desc_sw128(q_smem + t * S::kQ + (k >> 2) * (kRowsTile * 128) + (k & 3) * 32, 16),
                                desc_sw128(k_smem + (k >> 2) * (kN * 128) + (k & 3) * 32, 16), kQkDesc, k > 0);
                 tc_commit(s_full(slot));
             }
         };
-        auto weigh = [&](int t, int slot, int blk, bool fresh) {   // O (+)= P V
-            const uint32_t v_smem = ring + (blk % S::kSlots) * S::kBlock;
+        auto weigh = [&](int t, int slot, int blk, bool fresh, bool closes) {   // O (+)= P V
+            const uint32_t v_smem = ring + (blk % S::kRing) * S::kBlock;
             if (lead) {
 #pragma unroll
                 for (int z = 0; z < TERMS; ++z) {
-                    const uint32_t p = tmem + kSlotCol + slot * 128 + (z ? 32 + 32 * z : 0);
+                    const uint32_t p = tmem + kSlotCol + slot * S::kSlotCols + (z ? 32 + 32 * z : 0);
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
                         mma_f16_ts(tmem + t * D, p + k * 8, desc_sw128(v_smem + k * 2048, kN * 128), kPvDesc,
                                    !(fresh && z == 0 && k == 0));
                 }
                 tc_commit(o_done(t));
+                if (closes) tc_commit(o_last(t));
             }
         };
         bool alive = true;
-        int ready = 0;                                     // ring blocks known to be full
-        auto have = [&](int blk) {                         // block number blk has landed
-            if (blk < ready) return true;
-            if (!wait(full(blk % S::kSlots), (blk / S::kSlots) & 1)) return false;
-            ready = blk + 1;
-            return true;
+        int keys_in = -1, values_in = -1;                  // last blocks of each that have been waited for
+        auto have = [&](int blk, int &in) {                // block number blk has landed
+            if (blk == in) return true;
+            in = blk;
+            return wait(full(blk % S::kRing), (blk / S::kRing) & 1);
         };
         auto free_block = [&](int blk) {
-            if (lead) tc_commit(empty(blk % S::kSlots));
+            if (lead) tc_commit(empty(blk % S::kRing));
         };
         for (long long u = line.begin; alive;) {
             const int first = line.first_unit(u), last = line.last_unit();
@@ -587,51 +649,44 @@ __global__ void __launch_bounds__((TileShape<D, E4M3, TERMS>::kThreads), 1) attn
                 }
             }
             if (!alive) break;
-            alive = have(at);
+            alive = have(at, keys_in);
             if (!alive) break;
             tc_fence_after();
 #pragma unroll
             for (int t = 0; t < kT; ++t)
-                if (first < end[t]) score(t, kT == 2 ? t : 0, at);
+                if (first < end[t]) score(t, t * kBuf, at);
             free_block(at);
             for (int j = first; j < last && alive; ++j, at += 2) {
-                const int v_blk = at + 1, k_blk = at + 2;
-                if constexpr (kT == 1) {
-                    const int slot = (j - first) & 1;
-                    if (j + 1 < last) {
-                        if (!have(k_blk)) { alive = false; break; }
-                        tc_fence_after();
-                        score(0, slot ^ 1, k_blk);
-                        free_block(k_blk);
-                    }
-                    if (!wait(p_full(slot), p_phase >> slot & 1) || !have(v_blk)) { alive = false; break; }
-                    p_phase ^= 1u << slot;
+                const int v_blk = at + 1, k_blk = at + 2, buf = kBuf == 2 ? (j - first) & 1 : 0;
+                auto next_scores = [&](int t) {            // of block j + 1
+                    if (j + 1 >= end[t]) return true;
+                    if (!have(k_blk, keys_in)) return false;
                     tc_fence_after();
-                    weigh(0, slot, v_blk, j == first);
-                } else {
+                    score(t, t * kBuf + (kBuf == 2 ? buf ^ 1 : 0), k_blk);
+                    return true;
+                };
+                if constexpr (kBuf == 2) {
 #pragma unroll
-                    for (int t = 0; t < kT; ++t) {
-                        if (alive && j < end[t]) {
-                            if (!wait(p_full(t), p_phase >> t & 1) || !have(v_blk)) {
-                                alive = false;
-                            } else {
-                                p_phase ^= 1u << t;
-                                tc_fence_after();
-                                weigh(t, t, v_blk, j == first);
-                            }
-                        }
-                        if (alive && j + 1 < end[t]) {
-                            if (!have(k_blk)) {
-                                alive = false;
-                            } else {
-                                tc_fence_after();
-                                score(t, t, k_blk);
-                            }
-                        }
-                    }
+                    for (int t = 0; t < kT; ++t) alive = alive && next_scores(t);
                     if (!alive) break;
                     if (j + 1 < last) free_block(k_blk);
                 }
+#pragma unroll
+                for (int t = 0; t < kT; ++t) {
+                    const int slot = t * kBuf + buf;
+                    if (alive && j < end[t]) {
+                        if (!wait(p_full(slot), p_phase >> slot & 1) || !have(v_blk, values_in)) {
+                            alive = false;
+                        } else {
+                            p_phase ^= 1u << slot;
+                            tc_fence_after();
+                            weigh(t, slot, v_blk, j == first, j + 1 == end[t]);
+                        }
+                    }
+                    if constexpr (kBuf == 1) alive = alive && next_scores(t);
+                }
+                if (!alive) break;
+                if (kBuf == 1 && j + 1 < last) free_block(k_blk);
                 free_block(v_blk);
             }
             u = line.behind();
@@ -691,24 +746,54 @@ __global__ void __launch_bounds__(TILES * 128) attn_join_kernel(const AttnArgs a
     }
 }
 
-template <int D, bool E4M3, int TERMS>
-void launch(const AttnArgs &a, int sms) {
-    using S = TileShape<D, E4M3, TERMS>;
+// The pool as a matrix of rows of dim values, read in boxes of `box` rows x 64 values.
+bool pool_map(CUtensorMap &map, const AttnArgs &a, const void *pool) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.kv.dim, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)a.kv.dim * 2};
+    const cuuint32_t boxes[2] = {64, (cuuint32_t)a.box}, steps[2] = {1, 1};
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(pool), dims, strides, boxes, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, Load LOAD, int TERMS>
+void launch(const AttnArgs &a, int sms, const CUtensorMap &k_map, const CUtensorMap &v_map) {
+    using S = TileShape<D, LOAD, TERMS>;
     static bool set = false;
     if (!set) {
-        TQ_CHECK(cudaFuncSetAttribute(attn_tile_kernel<D, E4M3, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        TQ_CHECK(cudaFuncSetAttribute(attn_tile_kernel<D, LOAD, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
         set = true;
     }
     JoinTile *joins = reinterpret_cast<JoinTile *>(a.part + (size_t)2 * sms * S::kTiles * (D + 2) * kRowsTile);
-    launch_pdl(attn_tile_kernel<D, E4M3, TERMS>, dim3(sms), dim3(S::kThreads), (size_t)S::kSmem, a, joins);
+    launch_pdl(attn_tile_kernel<D, LOAD, TERMS>, dim3(sms), dim3(S::kThreads), (size_t)S::kSmem, a, joins, k_map, v_map);
     TQ_LAUNCH_CHECK("attn_tile_kernel");
     launch_pdl(attn_join_kernel<D, S::kTiles, TERMS == 1>, dim3(sms, D / 16), dim3(S::kTiles * 128), 0, a, (const JoinTile *)joins);
     TQ_LAUNCH_CHECK("attn_join_kernel");
 }
 template <int D>
-void launch_dim(const AttnArgs &a, bool e4m3, int sms) {
-    if (a.out_bf16) e4m3 ? launch<D, true, 1>(a, sms) : launch<D, false, 1>(a, sms);
-    else e4m3 ? launch<D, true, 2>(a, sms) : launch<D, false, 3>(a, sms);
+void launch_dim(AttnArgs a, bool e4m3, int sms) {
+    CUtensorMap k_map{}, v_map{};
+    if (e4m3) {
+        a.out_bf16 ? launch<D, kRegsE4m3, 1>(a, sms, k_map, v_map) : launch<D, kRegsE4m3, 2>(a, sms, k_map, v_map);
+        return;
+    }
+    // boxes of rows inside one page, in whole swizzle patterns of 8 rows; rows are counted in 32 bits
+    const long long rows = (long long)a.kv.pages * a.kv.heads * a.kv.page_size;
+    a.box = 64;
+    while (a.box > 4 && a.kv.page_size % a.box) a.box /= 2;
+    a.rows = rows < 0x7fffffffll ? (int)rows : 0;
+    if (a.box >= 8 && a.rows && pool_map(k_map, a, a.kv.k) && pool_map(v_map, a, a.kv.v))
+        a.out_bf16 ? launch<D, kTma, 1>(a, sms, k_map, v_map) : launch<D, kTma, 3>(a, sms, k_map, v_map);
+    else
+        a.out_bf16 ? launch<D, kRegs, 1>(a, sms, k_map, v_map) : launch<D, kRegs, 3>(a, sms, k_map, v_map);
 }
 
 }  // namespace
