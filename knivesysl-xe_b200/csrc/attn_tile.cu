@@ -10,7 +10,9 @@
 //   load     the blocks of keys and values, page by page, into a ring in shared memory: one warp that
 //            issues TMA copies of 8 to 64 rows, or, where pages are no multiple of 8 or the cache is
 //            e4m3 (which becomes fp16 on the way), four warps through their registers
-//   mma      one warp: S = Q K^T and O += P V, and the barriers that free ring and rows
+//   mma      a warp per tile: S = Q K^T and O += P V, and the barriers that free the ring. Issuing the
+//            products of two tiles takes one thread longer (2060 clocks per 64 keys at dim 128) than the
+//            tensor core needs for them (1310)
 // O is rescaled only when a row's maximum grows by more than 2^8: until then probabilities are up to
 // 2^8 instead of 1, which costs no precision, and the rescaling pass over O hardly ever runs.
 //
@@ -46,8 +48,8 @@ struct TileShape {
     static constexpr int kTiles = D <= 128 ? 2 : 1;                 // row tiles of a CTA
     static constexpr int kRows = kRowsTile * kTiles;
     static constexpr int kKeys = 64;                                // of a block
-    // Score buffers of a tile. With two, the scores of block j + 1 are multiplied while the probabilities
-    // of block j are computed; more terms of P leave room for one only.
+    // Score buffers of a tile. With two, the scores of block j + 1 lie ready when the probabilities of
+    // block j are done; more terms of P leave room for one only.
     static constexpr int kBuf = kTiles == 1 || TERMS == 1 ? 2 : 1;
     static constexpr int kSlotCols = 256 / (kTiles * kBuf);
     static constexpr int kBlock = kKeys * D * 2;                    // bytes of keys, or of values
@@ -55,15 +57,16 @@ struct TileShape {
     static constexpr int kQ = kRowsTile * D * 2;                    // bytes of a tile's queries
     static constexpr int kSmem = kTiles * kQ + kRing * kBlock + 1024;
     static constexpr int kSoftmax = kTiles * 128;                   // threads
-    static constexpr int kThreads = kSoftmax + kLoadWarps * 32 + 32;
+    static constexpr int kThreads = kSoftmax + kLoadWarps * 32 + kTiles * 32;
 };
 
 // 128-byte swizzle: rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7), groups of 8 rows 1024
 // bytes apart (SBO). K-major operands step 32 bytes per k16; MN-major ones (values: the summed
 // dimension runs over rows) have their next 64 columns LBO bytes further on.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
+// desc_lo: the low word, start address and LBO; the rest is the same for all (SBO, version 1, swizzle).
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr & 0x3FFFFu) >> 4) | (lbo >> 4) << 16; }
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+    return (uint64_t)lo | (uint64_t)((1024u >> 4) | 1u << 14 | 2u << 29) << 32;
 }
 // kind::f16: D = f32, A and B fp16 or bf16; B may be MN-major
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool b_mn) {
@@ -198,11 +201,11 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
     const uint32_t landed = drained + 8;               // a block that the load warp has to complete itself
 
     if (tid == 0) {
-        mbar_init(drained, 1);
+        mbar_init(drained, kT);
         mbar_init(landed, 1);
         for (int i = 0; i < S::kRing; ++i) {
             mbar_init(full(i), S::kLoadWarps);
-            mbar_init(empty(i), 1);
+            mbar_init(empty(i), kT);
         }
         for (int i = 0; i < kScores; ++i) {
             mbar_init(s_full(i), 1);
@@ -597,105 +600,87 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
         }
     } else {
         // ================================ mma ====================================================
-        uint32_t p_phase = 0, q_phase = 0;                 // a bit per slot, per tile
-        int at = 0;                                        // ring blocks so far (keys and values alternate)
-        const bool lead = elect_one();
-        auto score = [&](int t, int slot, int blk) {       // S = Q K^T
-            const uint32_t k_smem = ring + (blk % S::kRing) * S::kBlock;
-            if (lead) {
+        // One thread does it all: what it spends between two products may be time that the tensor core waits.
+        const int t = warp - kMmaWarp;
+        if (elect_one()) {
+            auto hold = [&](uint32_t bar, uint32_t parity) {
+                if (mbar_try_wait(bar, parity)) return true;
+                if (*wait.gave_up) return false;
+                if (mbar_wait_slow(bar, parity, a.kv.status, 24, a.limit_ns)) return true;
+                *wait.gave_up = 1;
+                return false;
+            };
+            uint32_t p_phase = 0, q_phase = 0;             // a bit per score buffer; queries so far
+            int at = 0;                                    // ring blocks so far (keys and values alternate)
+            // descriptors: the word with the address, counted in 16 bytes; a block of the ring, or a tile's
+            // queries, is a whole number of those further on
+            const uint32_t q_lo = desc_lo(q_smem + t * S::kQ, 16), k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kN * 128);
+            auto score = [&](int slot, int blk) {          // S = Q K^T
+                const uint32_t kd = k_lo + (blk & (S::kRing - 1)) * (S::kBlock >> 4);
+                const uint32_t d = tmem + kSlotCol + slot * S::kSlotCols;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_f16_ss(tmem + kSlotCol + slot * S::kSlotCols,
-                               desc_sw128(q_smem + t * S::kQ + (k >> 2) * (kRowsTile * 128) + (k & 3) * 32, 16),
-                               desc_sw128(k_smem + (k >> 2) * (kN * 128) + (k & 3) * 32, 16), kQkDesc, k > 0);
+                    mma_f16_ss(d, desc_of(q_lo + (((k >> 2) * (kRowsTile * 128) + (k & 3) * 32) >> 4)),
+                               desc_of(kd + (((k >> 2) * (kN * 128) + (k & 3) * 32) >> 4)), kQkDesc, k > 0);
                 tc_commit(s_full(slot));
-            }
-        };
-        auto weigh = [&](int t, int slot, int blk, bool fresh, bool closes) {   // O (+)= P V
-            const uint32_t v_smem = ring + (blk % S::kRing) * S::kBlock;
-            if (lead) {
+            };
+            auto weigh = [&](int slot, int blk, bool fresh, bool closes) {   // O (+)= P V
+                const uint32_t vd = v_lo + (blk & (S::kRing - 1)) * (S::kBlock >> 4);
+                const uint32_t d = tmem + t * D, p = tmem + kSlotCol + slot * S::kSlotCols;
 #pragma unroll
-                for (int z = 0; z < TERMS; ++z) {
-                    const uint32_t p = tmem + kSlotCol + slot * S::kSlotCols + (z ? 32 + 32 * z : 0);
+                for (int z = 0; z < TERMS; ++z)
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
-                        mma_f16_ts(tmem + t * D, p + k * 8, desc_sw128(v_smem + k * 2048, kN * 128), kPvDesc,
-                                   !(fresh && z == 0 && k == 0));
-                }
+                        mma_f16_ts(d, p + (z ? 32 + 32 * z : 0) + k * 8, desc_of(vd + (k * 2048 >> 4)), kPvDesc,
+                                   z || k ? 1u : (fresh ? 0u : 1u));
                 tc_commit(o_done(t));
                 if (closes) tc_commit(o_last(t));
-            }
-        };
-        bool alive = true;
-        int keys_in = -1, values_in = -1;                  // last blocks of each that have been waited for
-        auto have = [&](int blk, int &in) {                // block number blk has landed
-            if (blk == in) return true;
-            in = blk;
-            return wait(full(blk % S::kRing), (blk / S::kRing) & 1);
-        };
-        auto free_block = [&](int blk) {
-            if (lead) tc_commit(empty(blk % S::kRing));
-        };
-        for (long long u = line.begin; alive;) {
-            const int first = line.first_unit(u), last = line.last_unit();
-            if (last <= first) break;
-            int end[kT];
-#pragma unroll
-            for (int t = 0; t < kT; ++t) {
-                end[t] = tile_end(t, last);
-                if (alive && first < end[t]) {
-                    alive = wait(q_full(t), q_phase >> t & 1);
-                    q_phase ^= 1u << t;
+            };
+            // Every block is waited for and given back, also those that only the other tile's rows see
+            auto have = [&](int blk) { return hold(full(blk & (S::kRing - 1)), (blk / S::kRing) & 1); };
+            auto free_block = [&](int blk) { tc_commit(empty(blk & (S::kRing - 1))); };
+            bool alive = true;
+            for (long long u = line.begin; alive;) {
+                const int first = line.first_unit(u), last = line.last_unit(), end = tile_end(t, last);
+                if (last <= first) break;
+                if (first < end) {
+                    alive = hold(q_full(t), q_phase & 1);
+                    ++q_phase;
                 }
-            }
-            if (!alive) break;
-            alive = have(at, keys_in);
-            if (!alive) break;
-            tc_fence_after();
-#pragma unroll
-            for (int t = 0; t < kT; ++t)
-                if (first < end[t]) score(t, t * kBuf, at);
-            free_block(at);
-            for (int j = first; j < last && alive; ++j, at += 2) {
-                const int v_blk = at + 1, k_blk = at + 2, buf = kBuf == 2 ? (j - first) & 1 : 0;
-                auto next_scores = [&](int t) {            // of block j + 1
-                    if (j + 1 >= end[t]) return true;
-                    if (!have(k_blk, keys_in)) return false;
+                // the first kBuf blocks' scores, then block by block: P V, and the scores of the block that
+                // takes over its buffer
+                for (int j = first; j < min(first + kBuf, last) && alive; ++j) {
+                    const int k_blk = at + 2 * (j - first);
+                    alive = have(k_blk);
                     tc_fence_after();
-                    score(t, t * kBuf + (kBuf == 2 ? buf ^ 1 : 0), k_blk);
-                    return true;
-                };
-                if constexpr (kBuf == 2) {
-#pragma unroll
-                    for (int t = 0; t < kT; ++t) alive = alive && next_scores(t);
-                    if (!alive) break;
-                    if (j + 1 < last) free_block(k_blk);
+                    if (alive && j < end) score(t * kBuf + (j - first), k_blk);
+                    free_block(k_blk);
                 }
-#pragma unroll
-                for (int t = 0; t < kT; ++t) {
-                    const int slot = t * kBuf + buf;
-                    if (alive && j < end[t]) {
-                        if (!wait(p_full(slot), p_phase >> slot & 1) || !have(v_blk, values_in)) {
-                            alive = false;
-                        } else {
-                            p_phase ^= 1u << slot;
-                            tc_fence_after();
-                            weigh(t, slot, v_blk, j == first, j + 1 == end[t]);
-                        }
+                for (int j = first; j < last && alive; ++j, at += 2) {
+                    const int v_blk = at + 1, k_blk = at + 2 * kBuf, buf = (j - first) & (kBuf - 1), slot = t * kBuf + buf;
+                    alive = have(v_blk);
+                    if (alive && j < end) {
+                        alive = hold(p_full(slot), p_phase >> buf & 1);
+                        p_phase ^= 1u << buf;
+                        tc_fence_after();
+                        if (alive) weigh(slot, v_blk, j == first, j + 1 == end);
                     }
-                    if constexpr (kBuf == 1) alive = alive && next_scores(t);
+                    free_block(v_blk);
+                    if (alive && j + kBuf < last) {
+                        alive = have(k_blk);
+                        tc_fence_after();
+                        if (alive && j + kBuf < end) score(slot, k_blk);
+                        free_block(k_blk);
+                    }
                 }
-                if (!alive) break;
-                if (kBuf == 1 && j + 1 < last) free_block(k_blk);
-                free_block(v_blk);
+                u = line.behind();
+                if (u >= line.end) break;
+                line.next();
             }
-            u = line.behind();
-            if (u >= line.end) break;
-            line.next();
+            // no product runs on and no arrival is under way when the CTA ends, whether or not a wait gave up
+            tc_commit(drained);
+            mbar_wait_bounded(drained, 0, a.kv.status, 24, a.limit_ns);
         }
-        // no product runs on and no arrival is under way when the CTA ends, whether or not a wait gave up
-        if (lead) tc_commit(drained);
-        mbar_wait_bounded(drained, 0, a.kv.status, 24, a.limit_ns);
         __syncwarp();
     }
     __syncthreads();
