@@ -442,7 +442,8 @@ typedef struct {
  * be columns of one wide matrix); all 16-byte aligned, the strides multiples of 4. q_heads = 0 with d_q and d_q_out
  * NULL: keys and values only. rope NULL: neither norm nor rotation. e4m3 values beyond +-448 scales become +-448.
  * Two requests that share a page must not both write to it in one call.
- * Returns 0, -1 (bad record), -2 (bad arguments), -3 (sizes outside the kernels' range), -4 (alignment). */
+ * Returns 0, -1 (bad record), -2 (bad arguments), -3 (sizes outside the kernels' range), -4 (alignment), -40 (the
+ * process's first call that needs device memory of the library's own, made while the stream is being captured). */
 int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq_rope_t *rope, const float *d_q,
                     size_t ldq, int q_heads, uint16_t *d_q_out, const float *d_k, size_t ldk, const float *d_v,
                     size_t ldv);
@@ -451,15 +452,14 @@ int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, cons
  * [tokens][ldo] of q_heads * dim values, fp32 (computed to fp32's precision throughout) or, with out_bf16, bf16
  * (probabilities rounded to bf16 on the way). The cache behind d_kv_len[r] and unused pages are never read into a
  * result, whatever they hold; a value that is not finite below d_kv_len[r] may reach all rows of request r.
- * Returns as x_kv_append, and -40 when the call would have to allocate its workspace (once, on the first call: 40 MB)
- * while the stream is being captured. */
+ * Returns as x_kv_append; the workspace that the first call makes is 40 MB whatever the sizes. */
 int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const uint16_t *d_q, int q_heads,
                      float scale, void *d_out, size_t ldo, int out_bf16);
 /* ys[i][t] = bases[i][t] + scale (x[t] A^T) B^T with the adapter d_adapter[t] of ws[i] (negative: none, the row is
  * bases[i][t]); up to 4 projections of one input, with the same K and number of adapters. x fp32 [T][K], bases and
  * ys fp32 [T][M]; bases[i] may be ys[i] (added in place) or NULL, as may bases (0). Products and sums are fp32's.
  * An adapter number beyond the pool or a rank out of range counts as none and leaves 10043 in tq_last_error(). The
- * scratch grows with T and the ranks (-40 while the stream is being captured). Other returns as x_kv_append. */
+ * scratch grows with T (up to 4096) and the ranks. Returns as x_kv_append. */
 int qwn_x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *const *ys, int count,
                    const float *d_x, const int32_t *d_adapter, int T);
 

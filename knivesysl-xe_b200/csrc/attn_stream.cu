@@ -196,30 +196,42 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
             if (key0 >= keys) continue;
             const uint32_t kb = ring_u + (b % S::kStages) * S::kBlockBytes;
 
-            // ---- scores of 16 keys: two n8 tiles
-            float sc[2][4];
+            // ---- scores of 16 keys: two n8 tiles, each in two sums (a product that adds to the last one's
+            // result waits for it)
+            float sc[2][4], sc2[2][4];
+            uint32_t kline[2];
+            int kswz[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
                 const int key = t * 8 + row_a;
-                const int swz = (((key & 1) << 2) | ((key >> 1) & 3)) & (kChunks - 1);
-                const uint32_t line = kb + key * S::kRowBytes;
-#pragma unroll
-                for (int j = 0; j < kGroups; ++j) {
-                    uint32_t w[4];
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                 : "r"(line + (((j * 4 + quad) ^ swz) << 4)));
-#pragma unroll
-                    for (int s = 0; s < kSteps; ++s) {
-                        if constexpr (E4M3)
-                            mma16816<true>(sc[t], qf[j * kSteps + s], e4m3_to_f16((uint16_t)w[s]),
-                                           e4m3_to_f16((uint16_t)(w[s] >> 16)));
-                        else
-                            mma16816<false>(sc[t], qf[j * kSteps + s], w[2 * s], w[2 * s + 1]);
-                    }
-                }
+                sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
+                sc2[t][0] = sc2[t][1] = sc2[t][2] = sc2[t][3] = 0.0f;
+                kswz[t] = (((key & 1) << 2) | ((key >> 1) & 3)) & (kChunks - 1);
+                kline[t] = kb + key * S::kRowBytes;
             }
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                uint32_t w[2][4];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(w[t][0]), "=r"(w[t][1]), "=r"(w[t][2]), "=r"(w[t][3])
+                                 : "r"(kline[t] + (((j * 4 + quad) ^ kswz[t]) << 4)));
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        float (&d)[4] = s & 1 ? sc2[t] : sc[t];
+                        if constexpr (E4M3)
+                            mma16816<true>(d, qf[j * kSteps + s], e4m3_to_f16((uint16_t)w[t][s]), e4m3_to_f16((uint16_t)(w[t][s] >> 16)));
+                        else
+                            mma16816<false>(d, qf[j * kSteps + s], w[t][2 * s], w[t][2 * s + 1]);
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) sc[t][x] += sc2[t][x];
             // ---- running maximum and probabilities
             const bool cut = key0 + kKeys - 1 > low;
             float p[2][4];
@@ -282,22 +294,21 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
                 uint32_t w[4];
                 ldmatrix_x4_trans(vline + (((j + (lane >> 4)) ^ vswz) << 4), w);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {          // chunk j + i: w[2i] keys 0-7, w[2i + 1] keys 8-15
-                    if constexpr (E4M3) {
-                        // a unit holds two neighbouring dims of a key; bytes 0, 2 and 1, 3 pair the keys
+                for (int k = 0; k < kTerms; ++k)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t sel = x ? 0x4431u : 0x4420u;
-                            const uint32_t b0 = e4m3_to_f16((uint16_t)__byte_perm(w[2 * i], 0, sel));
-                            const uint32_t b1 = e4m3_to_f16((uint16_t)__byte_perm(w[2 * i + 1], 0, sel));
+                    for (int i = 0; i < 2; ++i) {      // chunk j + i: w[2i] keys 0-7, w[2i + 1] keys 8-15
+                        if constexpr (E4M3) {
+                            // a unit holds two neighbouring dims of a key; bytes 0, 2 and 1, 3 pair the keys
 #pragma unroll
-                            for (int k = 0; k < kTerms; ++k) mma16816<true>(o[(j + i) * 2 + x], pf[k], b0, b1);
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t sel = x ? 0x4431u : 0x4420u;
+                                mma16816<true>(o[(j + i) * 2 + x], pf[k], e4m3_to_f16((uint16_t)__byte_perm(w[2 * i], 0, sel)),
+                                               e4m3_to_f16((uint16_t)__byte_perm(w[2 * i + 1], 0, sel)));
+                            }
+                        } else {
+                            mma16816<false>(o[j + i], pf[k], w[2 * i], w[2 * i + 1]);
                         }
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < kTerms; ++k) mma16816<false>(o[j + i], pf[k], w[2 * i], w[2 * i + 1]);
                     }
-                }
             }
         }
         cp_async_wait<0>();
@@ -467,6 +478,7 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     if ((long long)a.kv.tokens * q_heads > 0x7fffff00ll) return -3;
     if (!aligned16(d_q) || !aligned16(d_out) || ldo % (out_bf16 ? 8 : 4)) return -4;
     if (const int rc = attn_scratch(sm_count())) return rc;
+    if (!device_status_ready()) return -40;
     a.kv.status = device_status_word();
     a.q = d_q;
     a.out = d_out;

@@ -42,6 +42,7 @@ void ensure_act_scratch(int K);
 // Device status word for bounded waits inside kernels (0 = clean), and the wall-clock limit
 // of those waits in nanoseconds (tq_set_wait_limit_ms).
 int *device_status_word();
+bool device_status_ready();     // false: the word is not there yet, and the stream is being captured, when it cannot be made
 unsigned long long wait_limit_ns();
 
 // State of the fused all-gather (comm.cu): buffers and flag words of every rank as mapped

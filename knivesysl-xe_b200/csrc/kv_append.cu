@@ -251,6 +251,7 @@ int x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq
     if ((q_heads && (!aligned16(d_q) || !aligned16(d_q_out) || ldq % 4)) || !aligned16(d_k) || !aligned16(d_v) || ldk % 4 ||
         ldv % 4)
         return -4;
+    if (!device_status_ready()) return -40;
     a.kv.status = device_status_word();
     a.q = d_q;
     a.k = d_k;

@@ -81,6 +81,11 @@ void ensure_act_scratch(int K) {
     s.prepared_K = 0;
 }
 
+bool device_status_ready() {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    return g_status_dev || (cudaStreamIsCapturing(stream(), &st) == cudaSuccess && st == cudaStreamCaptureStatusNone);
+}
+
 int *device_status_word() {
     if (!g_status_dev) {
         g_status_dev = static_cast<int *>(tq_dev_alloc(sizeof(int), "status"));
