@@ -77,7 +77,7 @@ int tq_last_error(void);                   /* sticky: cudaError of the last fail
 /* Every wait inside a kernel (the mbarrier waits of the tcgen05 GEMM, the flag wait of the
  * fused all-gather) gives up after a wall-clock limit, records a status word and lets the
  * kernel return normally; tq_sync() then turns the status into tq_last_error() = 10000 +
- * code (10021-10024: tcgen05 pipeline, 10031: a rank's gather flag never arrived; 10041-10043 are no
+ * code (10021-10025: tcgen05 pipeline and bulk copies, 10031: a rank's gather flag never arrived; 10041-10043 are no
  * waits: device arrays that describe a batch hold something impossible, see tq_kv_batch_t). Data
  * produced by a call whose wait gave up is incomplete: check tq_last_error() after
  * tq_sync() before trusting gathered outputs. The limit is two seconds unless changed here

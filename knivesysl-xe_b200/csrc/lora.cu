@@ -16,6 +16,7 @@
 // dimension that is summed is read in the order that suits the loads: a lane takes 16 bytes (8
 // neighbouring values) of a row, its share of two k16 steps, the same on both sides.
 #include "kv.cuh"
+#include "tc.cuh"
 
 #include <algorithm>
 
@@ -24,8 +25,10 @@ namespace tq {
 namespace {
 
 constexpr int kW = 8;                 // warps of a CTA
-constexpr int kTok = 64;              // tokens of a tile
+constexpr int kTok = 64;              // tokens of a tile of the shrink kernel
+constexpr int kTokE = 32;             // and of the expand kernel
 constexpr int kMaxTokens = 4096;      // of a launch
+constexpr size_t kSmemMost = 232448 - 256;   // dynamic shared memory of a CTA, beside some static
 constexpr int kMaxRank = 256;
 
 struct LoraArgs {
@@ -50,12 +53,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // ---- the batch's tokens by adapter -------------------------------------------------------------
-// Adapter numbers as this kernel takes them: -1 (none) for anything outside the pool.
-__device__ __forceinline__ int adapter_of(const LoraArgs &a, int t) {
-    const int id = __ldg(a.adapter + t);
-    if (id >= a.adapters) atomicCAS(a.status, 0, kStatusAdapter);
-    return id >= 0 && id < a.adapters ? id : -1;
-}
 __device__ __forceinline__ int rank_of(const LoraArgs &a, int i, int id) {
     if (!a.rank[i]) return a.R[i];
     const int r = __ldg(a.rank[i] + id);
@@ -63,71 +60,98 @@ __device__ __forceinline__ int rank_of(const LoraArgs &a, int i, int id) {
     return r < 0 || r > a.R[i] ? 0 : r;
 }
 
-// The batch's tokens as tiles: group 0 is "none", group id + 1 adapter id; s_off[g] = first tile of group
-// g, s_id = the groups of the tokens, s_list = the tokens of the tile at hand, in ascending order, so
-// that every CTA sees the same tiles.
+// The batch's tokens as tiles of TOK: group 0 is "none", group id + 1 adapter id; s_off[g] = first tile
+// of group g, s_id = the groups of the tokens, s_list = the tokens of the tile at hand, in ascending order,
+// so that every CTA sees the same tiles.
+template <int TOK>
 struct Plan {
     int *s_off, *s_cnt, *s_list, *s_sum;
     uint16_t *s_id;
     __device__ Plan(const LoraArgs &a, uint8_t *smem) {
         s_list = reinterpret_cast<int *>(smem);
-        s_sum = s_list + kTok;
+        s_sum = s_list + TOK;
         s_off = s_sum + kW;
         s_cnt = s_off + a.adapters + 2;
         s_id = reinterpret_cast<uint16_t *>(s_cnt + a.adapters + 1);
     }
-    static size_t bytes(int adapters, int T) { return ((size_t)kTok + kW + 2 * adapters + 3) * 4 + ((size_t)T + 1) / 2 * 4; }
-    __device__ int tokens(int g, int tile) const { return min(kTok, s_cnt[g] - (tile - s_off[g]) * kTok); }
-};
-// All threads of the CTA.
-__device__ void make_plan(const LoraArgs &a, const Plan &p) {
-    const int groups = a.adapters + 1, lane = threadIdx.x & 31;
-    for (int g = threadIdx.x; g < groups; g += kW * 32) p.s_cnt[g] = 0;
-    __syncthreads();
-    for (int t0 = 0; t0 < a.T; t0 += kW * 32) {
-        const int t = t0 + threadIdx.x, g = t < a.T ? adapter_of(a, t) + 1 : -1;
-        if (g >= 0) p.s_id[t] = (uint16_t)g;
-        const unsigned same = __match_any_sync(0xffffffffu, g);
-        if (g >= 0 && lane == __ffs(same) - 1) atomicAdd(p.s_cnt + g, __popc(same));
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {                          // exclusive scan of the groups' tiles
-        int tiles = 0;
-        for (int g0 = 0; g0 <= groups; g0 += 32) {
-            const int g = g0 + lane, m = g < groups ? (p.s_cnt[g] + kTok - 1) / kTok : 0;
-            int sum = m;
-            for (int off = 1; off < 32; off <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, sum, off);
-                if (lane >= off) sum += o;
+    static size_t bytes(int adapters, int T) { return ((size_t)TOK + kW + 2 * adapters + 3) * 4 + ((size_t)T + 1) / 2 * 4; }
+    __device__ int tokens(int g, int tile) const { return min(TOK, s_cnt[g] - (tile - s_off[g]) * TOK); }
+
+    // All threads of the CTA, of which the first kW warps work. Loops are kept short: code that runs once per launch
+    // is fetched from far away, and unrolled it costs more than it saves.
+    __device__ void make(const LoraArgs &a) const {
+        const int groups = a.adapters + 1, lane = threadIdx.x & 31;
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) s_cnt[g] = 0;
+        __syncthreads();
+        if (threadIdx.x < kW * 32) {
+#pragma unroll 1
+            for (int t0 = threadIdx.x; t0 - lane < a.T; t0 += 4 * kW * 32) {
+                int id[4];                           // loads under way together
+#pragma unroll
+                for (int i = 0; i < 4; ++i) id[i] = t0 + i * kW * 32 < a.T ? __ldg(a.adapter + t0 + i * kW * 32) : -1;
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + i * kW * 32, v = id[0];
+                    id[0] = id[1];
+                    id[1] = id[2];
+                    id[2] = id[3];
+                    if (t - lane >= a.T) break;
+                    if (v >= a.adapters) atomicCAS(a.status, 0, kStatusAdapter);
+                    // 0 for anything outside the pool, -1 behind the last token
+                    const int g = t >= a.T ? -1 : (v >= 0 && v < a.adapters ? v + 1 : 0);
+                    if (g >= 0) s_id[t] = (uint16_t)g;
+                    // tokens of a request follow one another: the first of a run adds the run
+                    const int before = __shfl_up_sync(0xffffffffu, g, 1);
+                    const unsigned heads = __ballot_sync(0xffffffffu, lane == 0 || before != g), behind = heads & ~((2u << lane) - 1);
+                    if ((heads >> lane & 1) && g >= 0) atomicAdd(s_cnt + g, (behind ? __ffs(behind) - 1 : 32) - lane);
+                }
             }
-            if (g <= groups) p.s_off[g] = tiles + sum - m;
-            tiles += __shfl_sync(0xffffffffu, sum, 31);
         }
+        __syncthreads();
+        if (threadIdx.x < 32) {                      // exclusive scan of the groups' tiles
+            int tiles = 0;
+#pragma unroll 1
+            for (int g0 = 0; g0 <= groups; g0 += 32) {
+                const int g = g0 + lane, m = g < groups ? (s_cnt[g] + TOK - 1) / TOK : 0;
+                int sum = m;
+#pragma unroll 1
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, sum, off);
+                    if (lane >= off) sum += o;
+                }
+                if (g <= groups) s_off[g] = tiles + sum - m;
+                tiles += __shfl_sync(0xffffffffu, sum, 31);
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
-}
-// The tokens of a tile into s_list; all threads of the CTA, each warp over an eighth of the batch.
-__device__ void list_tile(const LoraArgs &a, const Plan &p, int g, int tile) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, skip = (tile - p.s_off[g]) * kTok;
-    const int span = ((a.T + kW * 32 - 1) / (kW * 32)) * 32, t0 = warp * span, t1 = min(a.T, t0 + span);
-    int n = 0;
-    for (int t = t0; t < t1; t += 32) n += __popc(__ballot_sync(0xffffffffu, t + lane < t1 && p.s_id[t + lane] == g));
-    __syncthreads();                                 // the list and the sums are no longer read
-    if (lane == 0) p.s_sum[warp] = n;
-    __syncthreads();
-    int at = -skip;
-    for (int w = 0; w < warp; ++w) at += p.s_sum[w];
-    for (int t = t0; t < t1 && at < kTok; t += 32) {
-        const bool hit = t + lane < t1 && p.s_id[t + lane] == g;
-        const unsigned votes = __ballot_sync(0xffffffffu, hit);
-        const int place = at + __popc(votes & ((1u << lane) - 1));
-        if (hit && place >= 0 && place < kTok) p.s_list[place] = t + lane;
-        at += __popc(votes);
+    // The tokens of a tile into s_list; all threads of the CTA, the first kW warps over an eighth of the batch each.
+    __device__ void list(const LoraArgs &a, int g, int tile) const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, skip = (tile - s_off[g]) * TOK;
+        const int chunks = (a.T + kW * 32 - 1) / (kW * 32);      // of 32 tokens, of a warp
+        const int t0 = warp * chunks * 32 + lane, t1 = warp < kW ? min(a.T + 31, t0 - lane + chunks * 32) : 0;
+        int n = 0;
+#pragma unroll 2
+        for (int t = t0; t - lane < t1; t += 32) n += __popc(__ballot_sync(0xffffffffu, t < a.T && s_id[t] == g));
+        __syncthreads();                             // the list and the sums are no longer read
+        if (warp < kW && lane == 0) s_sum[warp] = n;
+        __syncthreads();
+        int at = -skip;
+        for (int w = 0; w < min(warp, kW); ++w) at += s_sum[w];
+#pragma unroll 2
+        for (int t = t0; t - lane < t1 && at < TOK; t += 32) {
+            const bool hit = t < a.T && s_id[t] == g;
+            const unsigned votes = __ballot_sync(0xffffffffu, hit);
+            const int place = at + __popc(votes & ((1u << lane) - 1));
+            if (hit && place >= 0 && place < TOK) s_list[place] = t;
+            at += __popc(votes);
+        }
+        __syncthreads();
     }
-    __syncthreads();
-}
+};
 // The group of tile x: the last g with s_off[g] <= x.
-__device__ __forceinline__ int group_of(const LoraArgs &a, const Plan &p, int x) {
+template <int TOK>
+__device__ __forceinline__ int group_of(const LoraArgs &a, const Plan<TOK> &p, int x) {
     int lo = 0, hi = a.adapters + 1;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -162,19 +186,19 @@ __device__ __forceinline__ void cp_async16_shared(uint32_t dst, const void *src,
 __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     auto sums = [&](int w) { return reinterpret_cast<float (*)[kNB * 8 + 2]>(smem + w * kStages * kStageBytes); };   // over the rings
-    const Plan plan(a, smem + kW * kStages * kStageBytes);
+    const Plan<kTok> plan(a, smem + kW * kStages * kStageBytes);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, row = lane >> 2;
     const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
     pdl_wait();
     pdl_trigger();
-    make_plan(a, plan);
+    plan.make(a);
     const int tile0 = plan.s_off[1], tiles = plan.s_off[a.adapters + 1] - tile0;      // group 0 has no product
     const int width = a.hoff[a.count], K64 = (a.K + 63) / 64;
     const int per = a.count * a.splits;
     for (int task = blockIdx.x; task < tiles * per; task += gridDim.x) {
         const int tile = tile0 + task / per, i = task % per / a.splits, part = task % a.splits;
         const int g = group_of(a, plan, tile), id = g - 1, tokens = plan.tokens(g, tile);
-        if (task == (int)blockIdx.x || tile != tile0 + (task - (int)gridDim.x) / per) list_tile(a, plan, g, tile);
+        if (task == (int)blockIdx.x || tile != tile0 + (task - (int)gridDim.x) / per) plan.list(a, g, tile);
         const int rank = rank_of(a, i, id), R = a.R[i];
         const int k0 = (int)((long long)K64 * part / a.splits), k1 = (int)((long long)K64 * (part + 1) / a.splits);
         const int groups16 = (tokens + 15) / 16, slices = groups16 == 1 ? 8 : (groups16 == 2 ? 4 : 2);
@@ -291,92 +315,91 @@ __device__ __forceinline__ uint4 first_values(uint4 v, int n) {
 }
 
 // ---- expand ------------------------------------------------------------------------------------
-// A task is (tile, projection, 256 columns of y): 32 columns a warp, whose rows of B (up to 64 ranks)
-// stay in registers while the tile's groups of 16 tokens go by, the next group's base rows under way.
-// h of the tile, scaled and split into its terms, lies in shared memory as [term][token][rank].
-constexpr int kCols = 32 * kW;
-__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// A task is (tile of 32 tokens, projection, block of columns): 256 columns with up to 64 ranks, 128 or
+// 64 with more, so that a block of B, which is one piece of memory, has at most 32 KB. A warp of its own
+// brings the block of B and the tokens' base rows (1 KB each) into a stage of shared memory by bulk
+// copies, up to three tasks ahead; the sixteen others multiply 32 columns by 16 tokens each, add and
+// store. So 130 KB an SM are under way whatever the products do. h of the tile, scaled and split into its terms, lies in shared memory
+// as [term][token][rank].
+constexpr int kWE = 16;                           // warps that multiply
+constexpr int kThreadsE = kWE * 32 + 32;
+constexpr int kRowPitch = 1024 + 64;              // bytes of a token's row in a stage: rows of 8 lanes on different banks
+constexpr int kBBytes = 32768;
+constexpr int kTaskBytes = kTokE * kRowPitch + kBBytes;
+__host__ __device__ inline int task_cols(int R) { return R <= 64 ? 256 : (R <= 128 ? 128 : 64); }
+__host__ __device__ inline int task_blocks(int M, int R) { return (M + task_cols(R) - 1) / task_cols(R); }
 // The column that row `row` of a warp's n8 tile n stands for: a lane's results in tiles 2i and 2i + 1 are
 // four neighbouring columns.
 __device__ __forceinline__ int column(int n, int row) { return (n >> 1) * 16 + (row >> 1) * 4 + (n & 1) * 2 + (row & 1); }
-
-__global__ void __launch_bounds__(kW * 32, 2) lora_expand_kernel(const LoraArgs a, int pitch) {
-    extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(kThreadsE, 1) lora_expand_kernel(const LoraArgs a, int pitch, int stages, unsigned long long limit_ns) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t s_bar[6];
+    __shared__ int s_gave_up;
     // pitch: ranks rounded up to 32, and 8 more: the rows of 8 lanes lie on different banks
-    uint16_t *const s_h = reinterpret_cast<uint16_t *>(smem);
-    const int plane = kTok * pitch;
-    const Plan plan(a, smem + (size_t)3 * plane * 2);
+    uint16_t *const s_h = reinterpret_cast<uint16_t *>(smem + stages * kTaskBytes);
+    const int plane = kTokE * pitch;
+    const Plan<kTokE> plan(a, reinterpret_cast<uint8_t *>(s_h + 3 * plane));
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, row = lane >> 2;
+    const uint32_t stage0 = smem_u32(smem), bars = smem_u32(s_bar);
+    auto full = [&](int s) { return bars + 8 * s; };             // a stage holds its task's operands
+    auto done = [&](int s) { return bars + 8 * (3 + s); };       // and they have been read
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 3; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(done(s), kWE);
+        }
+        mbar_init_fence();
+        s_gave_up = 0;
+    }
     pdl_wait();
     pdl_trigger();
-    make_plan(a, plan);
+    plan.make(a);
     const int tiles = plan.s_off[a.adapters + 1], width = a.hoff[a.count];
     int blocks = 0;
-    for (int i = 0; i < a.count; ++i) blocks += (a.M[i] + kCols - 1) / kCols;
-    const int total = tiles * blocks;                // below 2^31: 2112 tiles at most, of 2^15 blocks (checked by the entry point)
+    for (int i = 0; i < a.count; ++i) blocks += task_blocks(a.M[i], a.R[i]);
+    const int total = tiles * blocks;                // below 2^31 (checked by the entry point)
     const int begin = (int)((long long)total * blockIdx.x / gridDim.x), end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
-    int tile = begin / blocks, c = begin % blocks, i = 0, have_tile = -1, have_i = -1, rank = 0, g = 0;
-    while (c >= (a.M[i] + kCols - 1) / kCols) c -= (a.M[i++] + kCols - 1) / kCols;
-    for (int task = begin; task < end; ++task, ++c) {
-        if (c == (a.M[i] + kCols - 1) / kCols) {
-            c = 0;
-            if (++i == a.count) {
-                i = 0;
-                ++tile;
-            }
+    int tile = begin / max(1, blocks), c = begin % max(1, blocks), i = 0, have_tile = -1, g = 0;
+    while (c >= task_blocks(a.M[i], a.R[i])) c -= task_blocks(a.M[i], a.R[i++]);
+    int at = 0, loaded = 0;                          // tasks so far (stage at % stages), and those begun to load
+    bool alive = true;
+    auto hold = [&](uint32_t bar, uint32_t parity) { // by a whole warp
+        if (mbar_test_wait_warp(bar, parity)) return true;
+        bool ok = false;
+        if (!*(volatile int *)&s_gave_up) {
+            ok = mbar_wait_slow(bar, parity, a.status, 25, limit_ns);
+            if (!ok) *(volatile int *)&s_gave_up = 1;
         }
+        return (bool)__all_sync(0xffffffffu, ok);
+    };
+    // runs of tasks of one tile and projection
+    for (int task = begin; task < end;) {
+        const int cols = task_cols(a.R[i]), n = min(end - task, task_blocks(a.M[i], a.R[i]) - c);
         if (tile != have_tile) g = group_of(a, plan, tile);
-        const int id = g - 1, tokens = plan.tokens(g, tile);
-        if (id < 0 && a.base[i] == a.y[i]) continue;
-        const int R = a.R[i], M = a.M[i], col0 = c * kCols + warp * 32;
-        const bool fresh = tile != have_tile || i != have_i;       // another tile or projection: its h
-        if (fresh) {
-            if (tile != have_tile) list_tile(a, plan, g, tile);
+        const int id = g - 1, tokens = plan.tokens(g, tile), R = a.R[i], M = a.M[i];
+        const float *base = a.base[i];
+        float *const y = a.y[i];
+        if (id >= 0 || base != y) {
+            if (tile != have_tile) plan.list(a, g, tile);
+            else __syncthreads();                    // h is no longer read
             have_tile = tile;
-            have_i = i;
-            rank = id < 0 ? 0 : rank_of(a, i, id);
-        }
-        // the next task's rows of B and base, into L2: a line of 128 bytes per lane and row
-        if (col0 + kCols < M) {
-            if (rank) prefetch_l2(a.b[i] + ((size_t)id * M + min(M - 1, col0 + kCols + lane)) * R);
-            if (a.base[i])
-                for (int t = lane; t < tokens; t += 32) prefetch_l2(a.base[i] + (size_t)plan.s_list[t] * M + col0 + kCols);
-        }
-        // B of the warp's columns, ranks r0 .. r0 + 63
-        const bool odd = rank & 7;                   // a rank that ends inside a lane's 16 bytes
-        auto load_b = [&](int r0, uint4 (&w)[2][4]) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const int m = col0 + column(n, row), r = r0 + s * 32 + quad * 8;
-                    w[s][n] = m < M && r < rank ? __ldg(reinterpret_cast<const uint4 *>(a.b[i] + ((size_t)id * M + m) * R + r))
-                                                : make_uint4(0, 0, 0, 0);
-                    if (odd && r + 8 > rank) w[s][n] = first_values(w[s][n], rank - r);
-                }
-        };
-        auto load_base = [&](int m16, float4 (&v)[2][2]) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int tok = m16 * 16 + row + 8 * h;
-                const float *src = a.base[i] && tok < tokens ? a.base[i] + (size_t)plan.s_list[tok] * M : nullptr;
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int col = col0 + n * 16 + quad * 4;
-                    v[n][h] = src && col < M ? *reinterpret_cast<const float4 *>(src + col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-            }
-        };
-        uint4 w[2][4];
-        load_b(0, w);
-        float4 base[2][2];
-        load_base(0, base);
-        if (fresh) {
-            __syncthreads();
-            const int pad = (rank + 31) & ~31;
+            const int rank = id < 0 ? 0 : rank_of(a, i, id);
+            const uint16_t *B = a.b[i] + (size_t)max(id, 0) * M * R;
+            auto load = [&](int k) {                 // operands of the run's task k (warp kWE)
+                const int s = (at + k) % stages, col0 = (c + k) * cols, w = min(cols, M - col0);
+                const uint32_t dst = stage0 + s * kTaskBytes;
+                loaded = at + k + 1;
+                if (lane == 0) mbar_expect_tx(full(s), (base ? tokens * w * 4 : 0) + (rank ? w * R * 2 : 0));
+                __syncwarp();
+                if (rank && lane == 0) bulk_g2s_plain(dst + kTokE * kRowPitch, B + (size_t)col0 * R, w * R * 2, full(s));
+                if (base && lane < tokens) bulk_g2s_plain(dst + lane * kRowPitch, base + (size_t)plan.s_list[lane] * M + col0, w * 4, full(s));
+            };
+            if (warp == kWE)
+                for (int k = 0; k < min(stages, n) && alive; ++k) load(k);
+            // h of the tile
+            const int pad = (rank + 31) & ~31, rows16 = (tokens + 15) & ~15;
             const float scale = id < 0 ? 0.0f : (a.scale[i] ? __ldg(a.scale[i] + id) : 1.0f);
-            const int rows16 = (tokens + 15) & ~15;
-            for (int e = threadIdx.x; e < rows16 * (pad / 2); e += kW * 32) {
+            for (int e = threadIdx.x; e < rows16 * (pad / 2); e += kThreadsE) {
                 const int i_tok = e / (pad / 2), r = e % (pad / 2) * 2;
                 float v[2] = {0.0f, 0.0f};
                 if (i_tok < tokens && r < rank) {
@@ -401,50 +424,82 @@ __global__ void __launch_bounds__(kW * 32, 2) lora_expand_kernel(const LoraArgs 
                 dst[plane] = t2;
             }
             __syncthreads();
-        }
-        for (int m16 = 0; m16 * 16 < tokens; ++m16) {
-            float4 now[2][2];
+            if (warp == kWE) {
+                for (int k = 0; k < n && alive; ++k) {
+                    const int s = (at + k) % stages;
+                    alive = hold(done(s), ((at + k) / stages) & 1);
+                    if (alive && k + stages < n) load(k + stages);
+                }
+            } else {
+                const int across = cols / 32, wc = warp % across * 32, w16 = warp / across, step16 = kWE / across;
+                const bool odd = rank & 7;           // a rank that ends inside a lane's 16 bytes
+                for (int k = 0; k < n && alive; ++k) {
+                    const int s = (at + k) % stages, w = min(cols, M - (c + k) * cols);
+                    const uint8_t *const rows = smem + s * kTaskBytes;
+                    const uint8_t *const bs = rows + kTokE * kRowPitch;
+                    alive = hold(full(s), ((at + k) / stages) & 1);
+                    if (!alive) break;
+                    for (int m16 = w16; m16 * 16 < tokens; m16 += step16) {
+                        float acc[4][4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                now[n][0] = base[n][0];
-                now[n][1] = base[n][1];
-            }
-            if ((m16 + 1) * 16 < tokens) load_base(m16 + 1, base);
-            float acc[4][4];
+                        for (int q = 0; q < 4; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
+                        for (int r0 = 0; r0 < rank; r0 += 32) {
+                            uint4 b[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-            for (int r0 = 0; r0 < rank; r0 += 64) {
-                if (rank > 64) load_b(r0, w);
+                            for (int q = 0; q < 4; ++q) {
+                                const int m = wc + column(q, row), r = r0 + quad * 8;
+                                b[q] = m < w && r < rank ? *reinterpret_cast<const uint4 *>(bs + ((size_t)m * R + r) * 2) : make_uint4(0, 0, 0, 0);
+                                if (odd && r + 8 > rank) b[q] = first_values(b[q], rank - r);
+                            }
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    if (r0 + s * 32 >= rank) break;
+                            for (int z = 0; z < 3; ++z) {
+                                const uint16_t *hp = s_h + z * plane + (m16 * 16 + row) * pitch + r0 + quad * 8;
+                                const uint4 lo = *reinterpret_cast<const uint4 *>(hp), hi = *reinterpret_cast<const uint4 *>(hp + 8 * pitch);
+                                const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
-                    for (int z = 0; z < 3; ++z) {
-                        const uint16_t *hp = s_h + z * plane + (m16 * 16 + row) * pitch + r0 + s * 32 + quad * 8;
-                        const uint4 lo = *reinterpret_cast<const uint4 *>(hp), hi = *reinterpret_cast<const uint4 *>(hp + 8 * pitch);
-                        const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
+                                for (int q = 0; q < 4; ++q) mma_bf16(acc[q], f0, b[q].x, b[q].y);
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) mma_bf16(acc[n], f0, w[s][n].x, w[s][n].y);
+                                for (int q = 0; q < 4; ++q) mma_bf16(acc[q], f1, b[q].z, b[q].w);
+                            }
+                        }
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) mma_bf16(acc[n], f1, w[s][n].z, w[s][n].w);
+                        for (int h = 0; h < 2; ++h) {
+                            const int tok = m16 * 16 + row + 8 * h;
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const int col = wc + q * 16 + quad * 4;
+                                if (tok >= tokens || col >= w) continue;
+                                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                if (base) v = *reinterpret_cast<const float4 *>(rows + tok * kRowPitch + col * 4);
+                                v.x += acc[2 * q][2 * h];
+                                v.y += acc[2 * q][2 * h + 1];
+                                v.z += acc[2 * q + 1][2 * h];
+                                v.w += acc[2 * q + 1][2 * h + 1];
+                                *reinterpret_cast<float4 *>(y + (size_t)plan.s_list[tok] * M + (c + k) * cols + col) = v;
+                            }
+                        }
                     }
+                    __syncwarp();                    // all lanes have read the stage
+                    if (lane == 0) mbar_arrive(done(s));
                 }
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int tok = m16 * 16 + row + 8 * h;
-                if (tok >= tokens) continue;
-                float *dst = a.y[i] + (size_t)plan.s_list[tok] * M;
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int col = col0 + n * 16 + quad * 4;
-                    const float4 v = now[n][h];
-                    if (col < M)
-                        *reinterpret_cast<float4 *>(dst + col) =
-                            make_float4(v.x + acc[2 * n][2 * h], v.y + acc[2 * n][2 * h + 1], v.z + acc[2 * n + 1][2 * h], v.w + acc[2 * n + 1][2 * h + 1]);
-                }
+            at += n;
+        }
+        task += n;
+        c += n;
+        if (c == task_blocks(M, R)) {
+            c = 0;
+            if (++i == a.count) {
+                i = 0;
+                ++tile;
             }
         }
+        if (*(volatile int *)&s_gave_up) alive = false;
+    }
+    if (warp == kWE) {
+        if (!alive)                                  // a wait gave up: the copies under way end before the CTA does
+            for (int k = max(0, loaded - stages); k < loaded; ++k)
+                mbar_wait_bounded(full(k % stages), (k / stages) & 1, a.status, 25, limit_ns);
     }
 }
 
@@ -513,19 +568,22 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
     if (!device_status_ready()) return -40;
     a.status = device_status_word();
     int most = 0;
-    long long cols = 0;
+    long long blocks = 0;
     for (int i = 0; i < count; ++i) {
         most = std::max(most, a.R[i]);
-        cols += (a.M[i] + kCols - 1) / kCols;
+        blocks += task_blocks(a.M[i], a.R[i]);
     }
+    const int tiles_e = (piece + kTokE - 1) / kTokE + std::min(piece, a.adapters + 1);
+    if (blocks * tiles_e > 0x7fffffffll) return -3;
     const int pitch = ((most + 31) & ~31) + 8;
-    const size_t plan = Plan::bytes(a.adapters, piece);
-    const size_t shrink_smem = (size_t)kW * kStages * kStageBytes + plan;
-    const size_t expand_smem = (size_t)3 * kTok * pitch * 2 + plan;
+    const size_t shrink_smem = (size_t)kW * kStages * kStageBytes + Plan<kTok>::bytes(a.adapters, piece);
+    const size_t rest = (size_t)3 * kTokE * pitch * 2 + Plan<kTokE>::bytes(a.adapters, piece);
+    const int stages = 3 * kTaskBytes + rest <= kSmemMost ? 3 : 2;
+    const size_t expand_smem = stages * kTaskBytes + rest;
     static bool set = false;
     if (!set) {
-        TQ_CHECK(cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
-        TQ_CHECK(cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+        TQ_CHECK(cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
+        TQ_CHECK(cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
         set = true;
     }
     for (int t0 = 0; t0 < T; t0 += kMaxTokens) {
@@ -537,9 +595,9 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
             a.y[i] = ys[i] + (size_t)t0 * a.M[i];
         }
         const int shrink = (int)std::min<long long>((long long)tiles * count * a.splits, sms);
-        const int expand = (int)std::min<long long>(tiles * cols, 2 * sms);
+        const int expand = (int)std::min<long long>(tiles_e * blocks, sms);
         launch_pdl(lora_shrink_kernel, dim3(shrink), dim3(kW * 32), shrink_smem, a);
-        launch_pdl(lora_expand_kernel, dim3(expand), dim3(kW * 32), expand_smem, a, pitch);
+        launch_pdl(lora_expand_kernel, dim3(expand), dim3(kThreadsE), expand_smem, a, pitch, stages, wait_limit_ns());
     }
     TQ_LAUNCH_CHECK("lora_expand_kernel");
     return 0;
