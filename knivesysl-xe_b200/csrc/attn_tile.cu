@@ -27,8 +27,6 @@
 #include "attn.cuh"
 #include "tc.cuh"
 
-#include <cuda.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -731,24 +729,6 @@ __global__ void __launch_bounds__(TILES * 128) attn_join_kernel(const AttnArgs a
     }
 }
 
-// The pool as a matrix of rows of dim values, read in boxes of `box` rows x 64 values.
-bool pool_map(CUtensorMap &map, const AttnArgs &a, const void *pool) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess)
-            f = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-    }();
-    if (!encode) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)a.kv.dim, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)a.kv.dim * 2};
-    const cuuint32_t boxes[2] = {64, (cuuint32_t)a.box}, steps[2] = {1, 1};
-    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(pool), dims, strides, boxes, steps,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, Load LOAD, int TERMS>
 void launch(const AttnArgs &a, int sms, const CUtensorMap &k_map, const CUtensorMap &v_map) {
     using S = TileShape<D, LOAD, TERMS>;
@@ -775,7 +755,7 @@ void launch_dim(AttnArgs a, bool e4m3, int sms) {
     a.box = 64;
     while (a.box > 4 && a.kv.page_size % a.box) a.box /= 2;
     a.rows = rows < 0x7fffffffll ? (int)rows : 0;
-    if (a.box >= 8 && a.rows && pool_map(k_map, a, a.kv.k) && pool_map(v_map, a, a.kv.v))
+    if (a.box >= 8 && a.rows && tensor_map_2d(k_map, a.kv.k, D, rows, a.box) && tensor_map_2d(v_map, a.kv.v, D, rows, a.box))
         a.out_bf16 ? launch<D, kTma, 1>(a, sms, k_map, v_map) : launch<D, kTma, 3>(a, sms, k_map, v_map);
     else
         a.out_bf16 ? launch<D, kRegs, 1>(a, sms, k_map, v_map) : launch<D, kRegs, 3>(a, sms, k_map, v_map);

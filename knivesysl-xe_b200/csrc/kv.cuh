@@ -4,6 +4,8 @@
 
 #include "stream.cuh"
 
+#include <cuda.h>
+
 namespace tq {
 
 // Status words that a kernel leaves for tq_last_error() (10000 + code) when the batch's device
@@ -25,6 +27,9 @@ struct KvArgs {
 };
 // Checks the two records; 0 and the kernels' view of them, else the entry points' return code.
 int kv_args(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, KvArgs &a);
+// A bf16 matrix of rows of `cols` values (a multiple of 8, 16-byte aligned), for TMA copies of box_rows rows x 64
+// values with the 128-byte swizzle, zeros outside; false if the driver refuses it.
+bool tensor_map_2d(CUtensorMap &map, const void *data, int cols, long long rows, int box_rows);
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 #ifdef __CUDACC__

@@ -17,6 +17,7 @@
 #include "kv.cuh"
 
 #include <algorithm>
+#include <cudaTypedefs.h>
 
 namespace tq {
 
@@ -192,6 +193,23 @@ void launch(const AppendArgs &a, bool e4m3, dim3 grid) {
 bool stream_is_capturing() {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     return cudaStreamIsCapturing(stream(), &st) != cudaSuccess || st != cudaStreamCaptureStatusNone;
+}
+
+bool tensor_map_2d(CUtensorMap &map, const void *data, int cols, long long rows, int box_rows) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    if (!encode || rows >= 0x7fffffffll) return false;      // rows are counted in 32 bits
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols * 2};
+    const cuuint32_t boxes[2] = {64, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(data), dims, strides, boxes, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int kv_args(const tq_kv_cache_t *c, const tq_kv_batch_t *b, KvArgs &a) {

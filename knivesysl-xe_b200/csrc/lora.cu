@@ -4,13 +4,13 @@
 //
 // in two launches for up to four projections that share x: "shrink" h = x A^T (rank values a token)
 // and "expand" y = base + h B^T. Both work on tiles of up to 64 tokens of ONE adapter, whatever
-// places the tokens have in the batch: 16 of them are the m side of an mma, the adapter's rows the n
-// side, so an adapter is read once per 64 of its tokens and never for the others. Each CTA sorts the
+// places the tokens have in the batch, so an adapter is read once per 32 or 64 of its tokens and never
+// for the others. Each CTA sorts the
 // batch's adapter numbers into tiles itself (at most 4096 of a call's tokens at a time), which takes
 // it about a microsecond and spares a launch.
 //
 // Bytes bound both: x and the adapters in shrink, base, y and the adapters in expand; 2 rank
-// operations a value of x or y are far below that. x and h are fp32 and enter the bf16 tensor core
+// operations a value of x or y are below that. x and h are fp32 and enter the bf16 tensor core
 // as three bf16 terms, all 24 bits of them: exact up to the fp32 sums, which the tensor core cuts off
 // instead of rounding and which are therefore moved to ordinary fp32 sums every 128 values. The
 // dimension that is summed is read in the order that suits the loads: a lane takes 16 bytes (8
@@ -28,7 +28,7 @@ constexpr int kW = 8;                 // warps of a CTA
 constexpr int kTok = 64;              // tokens of a tile of the shrink kernel
 constexpr int kTokE = 32;             // and of the expand kernel
 constexpr int kMaxTokens = 4096;      // of a launch
-constexpr size_t kSmemMost = 232448 - 256;   // dynamic shared memory of a CTA, beside some static
+constexpr size_t kSmemMost = 232448 - 1024;   // dynamic shared memory of a CTA, beside some static
 constexpr int kMaxRank = 256;
 
 struct LoraArgs {
@@ -163,12 +163,13 @@ __device__ __forceinline__ int group_of(const LoraArgs &a, const Plan<TOK> &p, i
 
 // ---- shrink ------------------------------------------------------------------------------------
 // A task is (tile, projection, part of K). Its eight warps are shared out over the tile's 1 to 4 groups
-// of 16 tokens and, for each, slices of the part, whose sums are added through shared memory. A warp
-// brings 64 values of K of its 16 rows of x and of 64 ranks of A at a time through a ring of its own
-// (cp.async). Slices take turns at the 64 values, so that the CTA reads its rows in runs of 512 bytes or more.
+// of 16 tokens and, for each, slices of the part, whose sums are added through shared memory. The warps
+// of a slice bring 64 values of K at a time, each of its 16 rows of x and all together of 64 ranks of A,
+// through a ring of theirs (cp.async, 2 to 4 stages; one barrier of theirs a step). Slices take turns at
+// the 64 values, so that the CTA reads its rows in runs of 512 bytes or more.
 constexpr int kNB = 8;                // groups of 8 ranks per pass
-constexpr int kStages = 2;
-constexpr int kXBytes = 16 * 256, kABytes = kNB * 8 * 128, kStageBytes = kXBytes + kABytes;
+constexpr int kXBytes = 16 * 256, kABytes = kNB * 8 * 128;
+constexpr int kRingBytes = kW * 2 * (kXBytes + kABytes);          // of the CTA
 
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     uint4 v;
@@ -178,17 +179,12 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
 __device__ __forceinline__ void cp_async16_live(uint32_t dst, const void *src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
-// through L1, for what other warps of the CTA read at about the same time
-__device__ __forceinline__ void cp_async16_shared(uint32_t dst, const void *src, bool live) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
 
 __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
-    auto sums = [&](int w) { return reinterpret_cast<float (*)[kNB * 8 + 2]>(smem + w * kStages * kStageBytes); };   // over the rings
-    const Plan<kTok> plan(a, smem + kW * kStages * kStageBytes);
+    auto sums = [&](int w) { return reinterpret_cast<float (*)[kNB * 8 + 2]>(smem + w * (kRingBytes / kW)); };   // over the rings
+    const Plan<kTok> plan(a, smem + kRingBytes);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, row = lane >> 2;
-    const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
     pdl_wait();
     pdl_trigger();
     plan.make(a);
@@ -202,8 +198,10 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
         const int rank = rank_of(a, i, id), R = a.R[i];
         const int k0 = (int)((long long)K64 * part / a.splits), k1 = (int)((long long)K64 * (part + 1) / a.splits);
         const int groups16 = (tokens + 15) / 16, slices = groups16 == 1 ? 8 : (groups16 == 2 ? 4 : 2);
-        const int m = warp / slices, slice = warp % slices;    // m >= groups16: nothing to do (three groups)
-        const int steps = m < groups16 ? (k1 - k0 - slice + slices - 1) / slices : 0;
+        const int team = kW / slices, slice = warp / team, m = warp % team;    // m >= groups16: nothing to multiply (three groups)
+        const int steps = (k1 - k0 - slice + slices - 1) / slices;
+        const int stage_bytes = team * kXBytes + kABytes, stages = kRingBytes / slices / stage_bytes;      // 2, 3 or 4
+        const uint32_t ring = smem_u32(smem) + slice * (kRingBytes / slices);
         // this lane's chunks of x: rows 2 c + lane / 16, 16 bytes lane % 16 of 256
         int xt[8];
 #pragma unroll
@@ -216,37 +214,39 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
             const uint16_t *A = a.a[i] + ((size_t)id * R + r0) * a.K;
             auto issue = [&](int s) {
                 if (s < steps) {
-                    const uint32_t dst = ring + s % kStages * kStageBytes;
+                    const uint32_t dst = ring + s % stages * stage_bytes;
                     const int k = (k0 + slice + s * slices) * 64;
                     // K is a multiple of 32: the last 64 values may be 32
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         const int r = c * 2 + (lane >> 4), ch = lane & 15;
                         const bool live = xt[c] >= 0 && k + ch * 4 < a.K;
-                        cp_async16_live(dst + r * 256 + ((ch ^ (r & 1)) << 4), live ? a.x + (size_t)xt[c] * a.K + k + ch * 4 : a.x, live);
+                        cp_async16_live(dst + kABytes + m * kXBytes + r * 256 + ((ch ^ (r & 1)) << 4), live ? a.x + (size_t)xt[c] * a.K + k + ch * 4 : a.x, live);
                     }
-#pragma unroll
-                    for (int n = 0; n < kNB * 2; ++n)
-                        if (n < nb * 2) {
-                            const int r = n * 4 + (lane >> 3), ch = lane & 7;
-                            const bool live = r0 + r < rank && k + ch * 8 < a.K;
-                            cp_async16_shared(dst + kXBytes + r * 128 + ((ch ^ (r & 1) << 2) << 4), live ? A + (size_t)r * a.K + k + ch * 8 : A, live);
-                        }
+#pragma unroll 4
+                    for (int n = m; n < nb * 2; n += team) {
+                        const int r = n * 4 + (lane >> 3), ch = lane & 7;
+                        const bool live = r0 + r < rank && k + ch * 8 < a.K;
+                        cp_async16_live(dst + r * 128 + ((ch ^ (r & 1) << 2) << 4), live ? A + (size_t)r * a.K + k + ch * 8 : A, live);
+                    }
                 }
                 cp_async_commit();
             };
-#pragma unroll
-            for (int s = 0; s < kStages - 1; ++s) issue(s);
+            for (int s = 0; s < stages - 1; ++s) issue(s);
             float acc[kNB][4], sum[kNB][4];
 #pragma unroll
             for (int n = 0; n < kNB; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[n][e] = sum[n][e] = 0.0f;
             for (int s = 0; s < steps; ++s) {
-                issue(s + kStages - 1);
-                cp_async_wait<kStages - 1>();
-                __syncwarp();
-                const uint32_t src = ring + s % kStages * kStageBytes;
+                // stage s has landed when all but the stages - 2 copies behind it have
+                if (stages == 2) cp_async_wait<0>();
+                else if (stages == 3) cp_async_wait<1>();
+                else cp_async_wait<2>();
+                named_bar_sync(1 + slice, team * 32);     // for all warps of the team, which have read stage s - 1
+                issue(s + stages - 1);
+                if (m >= groups16) continue;
+                const uint32_t src = ring + s % stages * stage_bytes, xs = src + kABytes + m * kXBytes;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t f[2][3][4];                  // [k16 step][term]
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
                         const int r = row + 8 * h;
 #pragma unroll
                         for (int z = 0; z < 2; ++z) {
-                            const uint4 v = lds16(src + r * 256 + (((half * 8 + quad * 2 + z) ^ (r & 1)) << 4));
+                            const uint4 v = lds16(xs + r * 256 + (((half * 8 + quad * 2 + z) ^ (r & 1)) << 4));
                             split3(__uint_as_float(v.x), __uint_as_float(v.y), f[z][0][h], f[z][1][h], f[z][2][h]);
                             split3(__uint_as_float(v.z), __uint_as_float(v.w), f[z][0][2 + h], f[z][1][2 + h], f[z][2][2 + h]);
                         }
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
 #pragma unroll
                     for (int n = 0; n < kNB; ++n) {
                         const int r = n * 8 + row;
-                        if (n < nb) w[n] = lds16(src + kXBytes + r * 128 + (((half * 4 + quad) ^ (r & 1) << 2) << 4));
+                        if (n < nb) w[n] = lds16(src + r * 128 + (((half * 4 + quad) ^ (r & 1) << 2) << 4));
                     }
                     // neighbouring products go to different sums: one that needs the last one's waits for it
 #pragma unroll
@@ -286,10 +286,9 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
                             acc[n][e] = 0.0f;
                         }
                 }
-                __syncwarp();                             // all lanes have read the stage
             }
             cp_async_wait<0>();
-            __syncwarp();
+            __syncthreads();                              // the rings are free
 #pragma unroll
             for (int n = 0; n < kNB; ++n)
                 if (n < nb) {
@@ -300,7 +299,7 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
             for (int e = threadIdx.x; e < tokens * nb * 8; e += kW * 32) {
                 const int i_tok = e / (nb * 8), r = e % (nb * 8), t = plan.s_list[i_tok];
                 float s = 0.0f;
-                for (int w = 0; w < slices; ++w) s += sums((i_tok >> 4) * slices + w)[i_tok & 15][r];
+                for (int w = 0; w < slices; ++w) s += sums(w * team + (i_tok >> 4))[i_tok & 15][r];
                 a.h[((size_t)part * a.T + t) * width + a.hoff[i] + r0 + r] = s;
             }
             __syncthreads();
@@ -308,102 +307,140 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
     }
 }
 
-// The first n of 8 values, zeros behind them.
-__device__ __forceinline__ uint4 first_values(uint4 v, int n) {
-    auto word = [&](uint32_t x, int i) { return n >= 2 * i + 2 ? x : (n == 2 * i + 1 ? x & 0xffffu : 0u); };
-    return make_uint4(word(v.x, 0), word(v.y, 1), word(v.z, 2), word(v.w, 3));
+// ---- expand ------------------------------------------------------------------------------------
+// A task is (tile of 32 tokens, projection, 128 columns of y). The product is taken with the columns as
+// the tensor core's rows, D[128 columns][tokens] = B[128][ranks] h^T, so that a warp of the epilogue holds
+// 32 neighbouring columns of one token in its lanes: base and y are read and written in whole lines, and
+// per token a thread has one load, one addition and one store. (The same product on mma.sync took about
+// 1000 clocks a warp for every 16 x 16 results, twice what the memory needed.)
+//   load      one thread: 64 ranks of a task's rows of B by TMA into a ring of 16 KB stages, eight ahead
+//   mma       one thread: 12 products per 64 ranks (three terms of h), sums in tensor memory
+//   fix       one warp, for a rank that ends inside 16: zeros over what lies beyond it in the last product
+//   epilogue  two teams of four warps, which take turns at the tasks: the base rows are under way before
+//             the product is waited for
+// h of the tile, scaled and split into its terms, lies in shared memory as [64 ranks][term][token], rows of
+// 128 bytes with the 128-byte swizzle, as B does.
+constexpr int kCols = 128;
+constexpr int kRing = 8, kBlockB = kCols * 128;
+constexpr int kHTile = kTokE * 128;               // one term of 64 ranks of h
+constexpr int kAcc = 4;                           // accumulators of 32 columns in tensor memory
+constexpr int kThreadsE = 11 * 32;                // 8 warps epilogue, load, mma, fix
+
+struct LoraMaps {
+    CUtensorMap b[4];                             // B as rows [adapter x M] of rank values
+};
+
+// Whether tokens of a task are taken 16 or 32 at a time by the products.
+__device__ __forceinline__ uint32_t idesc_tokens(int n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kCols >> 4) << 24);
+}
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {       // K-major rows of 128 bytes, 128-byte swizzle
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
 }
 
-// ---- expand ------------------------------------------------------------------------------------
-// A task is (tile of 32 tokens, projection, block of columns): 256 columns with up to 64 ranks, 128 or
-// 64 with more, so that a block of B, which is one piece of memory, has at most 32 KB. A warp of its own
-// brings the block of B and the tokens' base rows (1 KB each) into a stage of shared memory by bulk
-// copies, up to three tasks ahead; the sixteen others multiply 32 columns by 16 tokens each, add and
-// store. So 130 KB an SM are under way whatever the products do. h of the tile, scaled and split into its terms, lies in shared memory
-// as [term][token][rank].
-constexpr int kWE = 16;                           // warps that multiply
-constexpr int kThreadsE = kWE * 32 + 32;
-constexpr int kRowPitch = 1024 + 64;              // bytes of a token's row in a stage: rows of 8 lanes on different banks
-constexpr int kBBytes = 32768;
-constexpr int kTaskBytes = kTokE * kRowPitch + kBBytes;
-__host__ __device__ inline int task_cols(int R) { return R <= 64 ? 256 : (R <= 128 ? 128 : 64); }
-__host__ __device__ inline int task_blocks(int M, int R) { return (M + task_cols(R) - 1) / task_cols(R); }
-// The column that row `row` of a warp's n8 tile n stands for: a lane's results in tiles 2i and 2i + 1 are
-// four neighbouring columns.
-__device__ __forceinline__ int column(int n, int row) { return (n >> 1) * 16 + (row >> 1) * 4 + (n & 1) * 2 + (row & 1); }
-__global__ void __launch_bounds__(kThreadsE, 1) lora_expand_kernel(const LoraArgs a, int pitch, int stages, unsigned long long limit_ns) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t s_bar[6];
+__global__ void __launch_bounds__(kThreadsE, 1)
+    lora_expand_kernel(const LoraArgs a, int chunks_max, unsigned long long limit_ns, const __grid_constant__ LoraMaps maps) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_bar[3 * kRing + 2 * kAcc + 1];
+    __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
-    // pitch: ranks rounded up to 32, and 8 more: the rows of 8 lanes lie on different banks
-    uint16_t *const s_h = reinterpret_cast<uint16_t *>(smem + stages * kTaskBytes);
-    const int plane = kTokE * pitch;
-    const Plan<kTokE> plan(a, reinterpret_cast<uint8_t *>(s_h + 3 * plane));
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, row = lane >> 2;
-    const uint32_t stage0 = smem_u32(smem), bars = smem_u32(s_bar);
-    auto full = [&](int s) { return bars + 8 * s; };             // a stage holds its task's operands
-    auto done = [&](int s) { return bars + 8 * (3 + s); };       // and they have been read
+    const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u, h_smem = ring + kRing * kBlockB;
+    const Plan<kTokE> plan(a, smem_raw + (ring - smem_u32(smem_raw)) + kRing * kBlockB + (size_t)chunks_max * 3 * kHTile);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t bars = smem_u32(s_bar);
+    auto full = [&](int i) { return bars + 8 * (i & (kRing - 1)); };                     // a stage has landed,
+    auto fixed = [&](int i) { return bars + 8 * (kRing + (i & (kRing - 1))); };          // has been mended (counted by themselves),
+    auto empty = [&](int i) { return bars + 8 * (2 * kRing + (i & (kRing - 1))); };      // may be written again
+    auto acc_full = [&](int i) { return bars + 8 * (3 * kRing + (i & (kAcc - 1))); };
+    auto acc_free = [&](int i) { return bars + 8 * (3 * kRing + kAcc + (i & (kAcc - 1))); };
+    const uint32_t drained = bars + 8 * (3 * kRing + 2 * kAcc);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 3; ++s) {
-            mbar_init(full(s), 1);
-            mbar_init(done(s), kWE);
+        for (int i = 0; i < 3 * kRing; ++i) mbar_init(bars + 8 * i, 1);
+        for (int i = 0; i < kAcc; ++i) {
+            mbar_init(acc_full(i), 1);
+            mbar_init(acc_free(i), 4);
         }
+        mbar_init(drained, 1);
         mbar_init_fence();
         s_gave_up = 0;
     }
-    pdl_wait();
-    pdl_trigger();
+    if (warp == 9) {
+        tmem_alloc(smem_u32(&s_tmem), kAcc * kTokE);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    // The shrink kernel lets this one start behind its own wait for all earlier kernels, so that everything but h
+    // may be read from here on.
     plan.make(a);
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
     const int tiles = plan.s_off[a.adapters + 1], width = a.hoff[a.count];
     int blocks = 0;
-    for (int i = 0; i < a.count; ++i) blocks += task_blocks(a.M[i], a.R[i]);
+    for (int i = 0; i < a.count; ++i) blocks += (a.M[i] + kCols - 1) / kCols;
     const int total = tiles * blocks;                // below 2^31 (checked by the entry point)
     const int begin = (int)((long long)total * blockIdx.x / gridDim.x), end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
-    int tile = begin / max(1, blocks), c = begin % max(1, blocks), i = 0, have_tile = -1, g = 0;
-    while (c >= task_blocks(a.M[i], a.R[i])) c -= task_blocks(a.M[i], a.R[i++]);
-    int at = 0, loaded = 0;                          // tasks so far (stage at % stages), and those begun to load
-    bool alive = true;
-    auto hold = [&](uint32_t bar, uint32_t parity) { // by a whole warp
-        if (mbar_test_wait_warp(bar, parity)) return true;
-        bool ok = false;
-        if (!*(volatile int *)&s_gave_up) {
-            ok = mbar_wait_slow(bar, parity, a.status, 25, limit_ns);
-            if (!ok) *(volatile int *)&s_gave_up = 1;
-        }
-        return (bool)__all_sync(0xffffffffu, ok);
+    int tile = begin / blocks, c = begin % blocks, i = 0, have_tile = -1, g = 0;
+    while (c >= (a.M[i] + kCols - 1) / kCols) c -= (a.M[i++] + kCols - 1) / kCols;
+    int at = 0, task_no = 0, fixes = 0;              // stages of B so far, tasks with a product, mended stages
+    auto hold = [&](uint32_t bar, uint32_t parity) { // by any threads of a warp
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*(volatile int *)&s_gave_up) return false;
+        if (mbar_wait_slow(bar, parity, a.status, 25, limit_ns)) return true;
+        *(volatile int *)&s_gave_up = 1;
+        return false;
     };
+    bool waited = false;
     // runs of tasks of one tile and projection
     for (int task = begin; task < end;) {
-        const int cols = task_cols(a.R[i]), n = min(end - task, task_blocks(a.M[i], a.R[i]) - c);
+        const int n = min(end - task, (a.M[i] + kCols - 1) / kCols - c);
         if (tile != have_tile) g = group_of(a, plan, tile);
-        const int id = g - 1, tokens = plan.tokens(g, tile), R = a.R[i], M = a.M[i];
+        const int id = g - 1, tokens = plan.tokens(g, tile), M = a.M[i];
         const float *base = a.base[i];
         float *const y = a.y[i];
         if (id >= 0 || base != y) {
             if (tile != have_tile) plan.list(a, g, tile);
-            else __syncthreads();                    // h is no longer read
+            else __syncthreads();                    // h and the list are no longer read
             have_tile = tile;
-            const int rank = id < 0 ? 0 : rank_of(a, i, id);
-            const uint16_t *B = a.b[i] + (size_t)max(id, 0) * M * R;
-            auto load = [&](int k) {                 // operands of the run's task k (warp kWE)
-                const int s = (at + k) % stages, col0 = (c + k) * cols, w = min(cols, M - col0);
-                const uint32_t dst = stage0 + s * kTaskBytes;
-                loaded = at + k + 1;
-                if (lane == 0) mbar_expect_tx(full(s), (base ? tokens * w * 4 : 0) + (rank ? w * R * 2 : 0));
-                __syncwarp();
-                if (rank && lane == 0) bulk_g2s_plain(dst + kTokE * kRowPitch, B + (size_t)col0 * R, w * R * 2, full(s));
-                if (base && lane < tokens) bulk_g2s_plain(dst + lane * kRowPitch, base + (size_t)plan.s_list[lane] * M + col0, w * 4, full(s));
-            };
-            if (warp == kWE)
-                for (int k = 0; k < min(stages, n) && alive; ++k) load(k);
-            // h of the tile
-            const int pad = (rank + 31) & ~31, rows16 = (tokens + 15) & ~15;
+            const int rank = id < 0 ? 0 : rank_of(a, i, id), chunks = (rank + 63) / 64;
+            const int fix = rank & 15;               // the last product of the last chunk has ranks that are not the adapter's
+            const int blk0 = at;
+            auto stage_of = [&](int k, int q) { return blk0 + k * chunks + q; };
+            if (warp == 8 && elect_one()) {
+                // ---- load
+                bool alive = true;
+                for (int x = 0; x < n * chunks && alive; ++x) {
+                    const int k = x / chunks, q = x % chunks, st = blk0 + x;
+                    if (st >= kRing) alive = hold(empty(st), ((st / kRing) - 1) & 1);
+                    if (!alive) break;
+                    mbar_expect_tx(full(st), kBlockB);
+                    tma_load_2d(ring + (st & (kRing - 1)) * kBlockB, &maps.b[i], q * 64, id * M + (c + k) * kCols, full(st));
+                }
+            }
+            __syncwarp();
+            // ---- h of the tile, by all
+            if (!waited) {
+                pdl_wait();
+                pdl_trigger();
+                waited = true;
+            }
             const float scale = id < 0 ? 0.0f : (a.scale[i] ? __ldg(a.scale[i] + id) : 1.0f);
-            for (int e = threadIdx.x; e < rows16 * (pad / 2); e += kThreadsE) {
-                const int i_tok = e / (pad / 2), r = e % (pad / 2) * 2;
+            for (int e = threadIdx.x; e < chunks * kTokE * 32; e += kThreadsE) {
+                const int tok = e >> 5 & (kTokE - 1), q = e / (kTokE * 32), r = q * 64 + (e & 31) * 2;
                 float v[2] = {0.0f, 0.0f};
-                if (i_tok < tokens && r < rank) {
-                    const float *h = a.h + (size_t)plan.s_list[i_tok] * width + a.hoff[i] + r;
+                if (tok < tokens && r < rank) {
+                    const float *h = a.h + (size_t)plan.s_list[tok] * width + a.hoff[i] + r;
                     float2 part[8];                  // at most 8 parts, all loads under way together
 #pragma unroll
                     for (int s = 0; s < 8; ++s)
@@ -416,91 +453,135 @@ __global__ void __launch_bounds__(kThreadsE, 1) lora_expand_kernel(const LoraArg
                 }
                 v[0] = r < rank ? v[0] * scale : 0.0f;
                 v[1] = r + 1 < rank ? v[1] * scale : 0.0f;
-                uint32_t t0, t1, t2;
-                split3(v[0], v[1], t0, t1, t2);
-                uint32_t *dst = reinterpret_cast<uint32_t *>(s_h + i_tok * pitch + r);
-                dst[0] = t0;
-                dst[plane / 2] = t1;
-                dst[plane] = t2;
+                uint32_t t[3];
+                split3(v[0], v[1], t[0], t[1], t[2]);
+                const uint32_t to = h_smem + q * 3 * kHTile + tok * 128 + (((e >> 2 & 7) ^ (tok & 7)) << 4) + (e & 3) * 4;
+#pragma unroll
+                for (int z = 0; z < 3; ++z) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + z * kHTile), "r"(t[z]) : "memory");
             }
+            fence_proxy_async_smem();
             __syncthreads();
-            if (warp == kWE) {
-                for (int k = 0; k < n && alive; ++k) {
-                    const int s = (at + k) % stages;
-                    alive = hold(done(s), ((at + k) / stages) & 1);
-                    if (alive && k + stages < n) load(k + stages);
-                }
-            } else {
-                const int across = cols / 32, wc = warp % across * 32, w16 = warp / across, step16 = kWE / across;
-                const bool odd = rank & 7;           // a rank that ends inside a lane's 16 bytes
-                for (int k = 0; k < n && alive; ++k) {
-                    const int s = (at + k) % stages, w = min(cols, M - (c + k) * cols);
-                    const uint8_t *const rows = smem + s * kTaskBytes;
-                    const uint8_t *const bs = rows + kTokE * kRowPitch;
-                    alive = hold(full(s), ((at + k) / stages) & 1);
-                    if (!alive) break;
-                    for (int m16 = w16; m16 * 16 < tokens; m16 += step16) {
-                        float acc[4][4];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) acc[q][0] = acc[q][1] = acc[q][2] = acc[q][3] = 0.0f;
-                        for (int r0 = 0; r0 < rank; r0 += 32) {
-                            uint4 b[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const int m = wc + column(q, row), r = r0 + quad * 8;
-                                b[q] = m < w && r < rank ? *reinterpret_cast<const uint4 *>(bs + ((size_t)m * R + r) * 2) : make_uint4(0, 0, 0, 0);
-                                if (odd && r + 8 > rank) b[q] = first_values(b[q], rank - r);
-                            }
-#pragma unroll
-                            for (int z = 0; z < 3; ++z) {
-                                const uint16_t *hp = s_h + z * plane + (m16 * 16 + row) * pitch + r0 + quad * 8;
-                                const uint4 lo = *reinterpret_cast<const uint4 *>(hp), hi = *reinterpret_cast<const uint4 *>(hp + 8 * pitch);
-                                const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) mma_bf16(acc[q], f0, b[q].x, b[q].y);
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) mma_bf16(acc[q], f1, b[q].z, b[q].w);
-                            }
+            if (warp == 9) {
+                // ---- mma
+                if (elect_one()) {
+                    const uint32_t idesc = idesc_tokens(tokens > 16 ? 32 : 16);
+                    bool alive = true;
+                    for (int k = 0; k < n && chunks && alive; ++k) {
+                        const int no = task_no + k;
+                        if (no >= kAcc) alive = hold(acc_free(no), ((no / kAcc) - 1) & 1);
+                        const uint32_t d = tmem + (no & (kAcc - 1)) * kTokE;
+                        for (int q = 0; q < chunks && alive; ++q) {
+                            const int st = stage_of(k, q);
+                            alive = fix && q == chunks - 1 ? hold(fixed(fixes + k), ((fixes + k) / kRing) & 1) : hold(full(st), (st / kRing) & 1);
+                            if (!alive) break;
+                            tc_fence_after();
+                            const uint32_t b_smem = ring + (st & (kRing - 1)) * kBlockB, hq = h_smem + q * 3 * kHTile;
+                            const int steps = min(4, (rank - q * 64 + 15) / 16);
+                            for (int z = 0; z < 3; ++z)
+                                for (int s = 0; s < steps; ++s)
+                                    mma_f16_ss(d, desc_sw128(b_smem + s * 32), desc_sw128(hq + z * kHTile + s * 32), idesc, q || z || s);
+                            tc_commit(empty(st));
                         }
+                        if (alive) tc_commit(acc_full(no));
+                    }
+                }
+                __syncwarp();                        // the warp comes to the barriers below as one
+            } else if (warp == 10) {
+                // ---- fix
+                bool alive = true;
+                for (int k = 0; k < n && fix && alive; ++k) {
+                    const int st = stage_of(k, chunks - 1), r0 = (rank & 63) & ~15;      // first rank of the last product, in its chunk
+                    alive = __all_sync(0xffffffffu, hold(full(st), (st / kRing) & 1));
+                    if (!alive) break;
+                    const uint32_t b_smem = ring + (st & (kRing - 1)) * kBlockB;
+#pragma unroll 1
+                    for (int x = lane; x < kCols * 2; x += 32) {
+                        const int m = x >> 1, ch = (r0 >> 3) + (x & 1), keep = fix - (x & 1) * 8;      // values of this chunk that are the adapter's
+                        if (keep >= 8) continue;
+                        const uint32_t at_m = b_smem + m * 128 + ((ch ^ (m & 7)) << 4);
+                        const uint4 v = lds16(at_m);
+                        auto word = [&](uint32_t w, int j) { return keep >= 2 * j + 2 ? w : (keep == 2 * j + 1 ? w & 0xffffu : 0u); };
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at_m), "r"(word(v.x, 0)), "r"(word(v.y, 1)), "r"(word(v.z, 2)),
+                                     "r"(word(v.w, 3))
+                                     : "memory");
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(fixed(fixes + k));
+                }
+            } else if (warp < 8) {
+                // ---- epilogue
+                bool alive = true;
+                for (int k = warp >> 2; k < n && alive; k += 2) {
+                    const int no = task_no + k, col = (c + k) * kCols + (warp & 3) * 32 + lane;
+                    const bool live = col < M;
+                    float v[kTokE];
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int tok = m16 * 16 + row + 8 * h;
+                    for (int t0 = 0; t0 < kTokE; t0 += 8) {
+                        if (t0 < tokens) {
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                const int col = wc + q * 16 + quad * 4;
-                                if (tok >= tokens || col >= w) continue;
-                                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                if (base) v = *reinterpret_cast<const float4 *>(rows + tok * kRowPitch + col * 4);
-                                v.x += acc[2 * q][2 * h];
-                                v.y += acc[2 * q][2 * h + 1];
-                                v.z += acc[2 * q + 1][2 * h];
-                                v.w += acc[2 * q + 1][2 * h + 1];
-                                *reinterpret_cast<float4 *>(y + (size_t)plan.s_list[tok] * M + (c + k) * cols + col) = v;
-                            }
+                            for (int t = t0; t < t0 + 8; ++t)
+                                v[t] = base && live && t < tokens ? base[(size_t)plan.s_list[t] * M + col] : 0.0f;
                         }
                     }
-                    __syncwarp();                    // all lanes have read the stage
-                    if (lane == 0) mbar_arrive(done(s));
+                    if (chunks) {
+                        alive = __all_sync(0xffffffffu, hold(acc_full(no), (no / kAcc) & 1));
+                        if (!alive) break;
+                        tc_fence_after();
+                        const uint32_t d = tmem + ((uint32_t)(warp & 3) << 21) + (no & (kAcc - 1)) * kTokE;
+#pragma unroll
+                        for (int t0 = 0; t0 < kTokE; t0 += 16) {
+                            if (t0 < tokens) {
+                                uint32_t w[16];
+                                tmem_ld16(d + t0, w);
+                                tmem_wait_ld16(w);
+#pragma unroll
+                                for (int t = 0; t < 16; ++t) v[t0 + t] += __uint_as_float(w[t]);
+                            }
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_free(no));
+                    }
+#pragma unroll
+                    for (int t0 = 0; t0 < kTokE; t0 += 8) {
+                        if (t0 < tokens) {
+#pragma unroll
+                            for (int t = t0; t < t0 + 8; ++t)
+                                if (live && t < tokens) y[(size_t)plan.s_list[t] * M + col] = v[t];
+                        }
+                    }
+                    __syncwarp();
                 }
             }
-            at += n;
+            at += n * chunks;
+            if (chunks) task_no += n;
+            if (fix) fixes += n;
         }
         task += n;
         c += n;
-        if (c == task_blocks(M, R)) {
+        if (c == (M + kCols - 1) / kCols) {
             c = 0;
             if (++i == a.count) {
                 i = 0;
                 ++tile;
             }
         }
-        if (*(volatile int *)&s_gave_up) alive = false;
     }
-    if (warp == kWE) {
-        if (!alive)                                  // a wait gave up: the copies under way end before the CTA does
-            for (int k = max(0, loaded - stages); k < loaded; ++k)
-                mbar_wait_bounded(full(k % stages), (k / stages) & 1, a.status, 25, limit_ns);
+    if (!waited) pdl_wait();
+    __syncthreads();
+    if (warp == 8 && s_gave_up && lane == 0)         // copies may still be under way: they end before the CTA does
+        for (int st = max(0, at - kRing); st < at; ++st) mbar_wait_bounded(full(st), (st / kRing) & 1, a.status, 25, limit_ns);
+    if (warp == 9) {
+        if (elect_one()) {
+            tc_commit(drained);
+            mbar_wait_bounded(drained, 0, a.status, 25, limit_ns);
+        }
+        __syncwarp();
     }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, kAcc * kTokE);
 }
 
 float *g_h = nullptr;
@@ -569,17 +650,17 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
     a.status = device_status_word();
     int most = 0;
     long long blocks = 0;
+    LoraMaps maps{};
     for (int i = 0; i < count; ++i) {
         most = std::max(most, a.R[i]);
-        blocks += task_blocks(a.M[i], a.R[i]);
+        blocks += (a.M[i] + kCols - 1) / kCols;
+        if (!tensor_map_2d(maps.b[i], a.b[i], a.R[i], (long long)a.adapters * a.M[i], kCols)) return -3;
     }
     const int tiles_e = (piece + kTokE - 1) / kTokE + std::min(piece, a.adapters + 1);
     if (blocks * tiles_e > 0x7fffffffll) return -3;
-    const int pitch = ((most + 31) & ~31) + 8;
-    const size_t shrink_smem = (size_t)kW * kStages * kStageBytes + Plan<kTok>::bytes(a.adapters, piece);
-    const size_t rest = (size_t)3 * kTokE * pitch * 2 + Plan<kTokE>::bytes(a.adapters, piece);
-    const int stages = 3 * kTaskBytes + rest <= kSmemMost ? 3 : 2;
-    const size_t expand_smem = stages * kTaskBytes + rest;
+    const int chunks = (most + 63) / 64;
+    const size_t shrink_smem = (size_t)kRingBytes + Plan<kTok>::bytes(a.adapters, piece);
+    const size_t expand_smem = 1024 + (size_t)kRing * kBlockB + (size_t)chunks * 3 * kHTile + Plan<kTokE>::bytes(a.adapters, piece);
     static bool set = false;
     if (!set) {
         TQ_CHECK(cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
@@ -597,7 +678,7 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
         const int shrink = (int)std::min<long long>((long long)tiles * count * a.splits, sms);
         const int expand = (int)std::min<long long>(tiles_e * blocks, sms);
         launch_pdl(lora_shrink_kernel, dim3(shrink), dim3(kW * 32), shrink_smem, a);
-        launch_pdl(lora_expand_kernel, dim3(expand), dim3(kThreadsE), expand_smem, a, pitch, stages, wait_limit_ns());
+        launch_pdl(lora_expand_kernel, dim3(expand), dim3(kThreadsE), expand_smem, a, chunks, wait_limit_ns(), maps);
     }
     TQ_LAUNCH_CHECK("lora_expand_kernel");
     return 0;
