@@ -314,24 +314,26 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
 // per token a thread has one load, one addition and one store. (The same product on mma.sync took about
 // 1000 clocks a warp for every 16 x 16 results, twice what the memory needed.)
 //   load      one thread: 64 ranks of a task's rows of B by TMA into a ring of 16 KB stages, eight ahead
-//   mma       one thread: 12 products per 64 ranks (three terms of h), sums in tensor memory
-//   fix       one warp, for a rank that ends inside 16: zeros over what lies beyond it in the last product
-//   epilogue  two teams of four warps, which take turns at the tasks: the base rows are under way before
-//             the product is waited for
+//   mma       one thread: 4 products per 64 ranks, h's three terms beside one another as columns
+//   fix       for a rank that ends inside 16: zeros over what lies beyond it in the last product (whatever B holds
+//             there must not get in). About a microsecond a task, mostly latency: four warps take tasks in turn
+//   epilogue  two teams of four warps, which take turns at the tasks, the base rows of the team's next task
+//             under way meanwhile
 // h of the tile, scaled and split into its terms, lies in shared memory as [64 ranks][term][token], rows of
-// 128 bytes with the 128-byte swizzle, as B does.
+// 128 bytes with the 128-byte swizzle, as B does. Up to 16 tokens it has 16 rows a term, else 32.
 constexpr int kCols = 128;
 constexpr int kRing = 8, kBlockB = kCols * 128;
-constexpr int kHTile = kTokE * 128;               // one term of 64 ranks of h
-constexpr int kAcc = 4;                           // accumulators of 32 columns in tensor memory
-constexpr int kThreadsE = 11 * 32;                // 8 warps epilogue, load, mma, fix
+constexpr int kHTile = 3 * kTokE * 128;           // 64 ranks of h, its three terms one below the other
+constexpr int kAcc = 4;                           // accumulators in tensor memory, of a column per term and token
+constexpr int kAccCols = 128;
+constexpr int kFixWarps = 4;
+constexpr int kThreadsE = (10 + kFixWarps) * 32;  // 8 warps epilogue, load, mma, fix
 
 struct LoraMaps {
     CUtensorMap b[4];                             // B as rows [adapter x M] of rank values
 };
 
-// Whether tokens of a task are taken 16 or 32 at a time by the products.
-__device__ __forceinline__ uint32_t idesc_tokens(int n) {
+__device__ __forceinline__ uint32_t idesc_cols(int n) {       // D f32 [128][n], A and B bf16, both K-major
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kCols >> 4) << 24);
 }
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {       // K-major rows of 128 bytes, 128-byte swizzle
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u, h_smem = ring + kRing * kBlockB;
-    const Plan<kTokE> plan(a, smem_raw + (ring - smem_u32(smem_raw)) + kRing * kBlockB + (size_t)chunks_max * 3 * kHTile);
+    const Plan<kTokE> plan(a, smem_raw + (ring - smem_u32(smem_raw)) + kRing * kBlockB + (size_t)chunks_max * kHTile);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t bars = smem_u32(s_bar);
     auto full = [&](int i) { return bars + 8 * (i & (kRing - 1)); };                     // a stage has landed,
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
         s_gave_up = 0;
     }
     if (warp == 9) {
-        tmem_alloc(smem_u32(&s_tmem), kAcc * kTokE);
+        tmem_alloc(smem_u32(&s_tmem), kAcc * kAccCols);
         tmem_relinquish();
         tc_fence_before();
     }
@@ -415,20 +417,23 @@ __global__ void __launch_bounds__(kThreadsE, 1)
             have_tile = tile;
             const int rank = id < 0 ? 0 : rank_of(a, i, id), chunks = (rank + 63) / 64;
             const int fix = rank & 15;               // the last product of the last chunk has ranks that are not the adapter's
-            const int blk0 = at;
+            const int blk0 = at, rows_term = tokens > 16 ? 32 : 16;
             auto stage_of = [&](int k, int q) { return blk0 + k * chunks + q; };
-            if (warp == 8 && elect_one()) {
-                // ---- load
+            // ---- load: stages [x0, x1) of the run; those of one ring need none of the run's own products
+            auto load = [&](int x0, int x1) {
                 bool alive = true;
-                for (int x = 0; x < n * chunks && alive; ++x) {
+                for (int x = x0; x < x1 && alive; ++x) {
                     const int k = x / chunks, q = x % chunks, st = blk0 + x;
                     if (st >= kRing) alive = hold(empty(st), ((st / kRing) - 1) & 1);
                     if (!alive) break;
                     mbar_expect_tx(full(st), kBlockB);
                     tma_load_2d(ring + (st & (kRing - 1)) * kBlockB, &maps.b[i], q * 64, id * M + (c + k) * kCols, full(st));
                 }
+            };
+            if (warp == 8) {
+                if (elect_one()) load(0, min(n * chunks, kRing));
+                __syncwarp();
             }
-            __syncwarp();
             // ---- h of the tile, by all
             if (!waited) {
                 pdl_wait();
@@ -436,8 +441,8 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                 waited = true;
             }
             const float scale = id < 0 ? 0.0f : (a.scale[i] ? __ldg(a.scale[i] + id) : 1.0f);
-            for (int e = threadIdx.x; e < chunks * kTokE * 32; e += kThreadsE) {
-                const int tok = e >> 5 & (kTokE - 1), q = e / (kTokE * 32), r = q * 64 + (e & 31) * 2;
+            for (int e = threadIdx.x; e < chunks * rows_term * 32; e += kThreadsE) {
+                const int tok = e >> 5 & (rows_term - 1), q = e / (rows_term * 32), r = q * 64 + (e & 31) * 2;
                 float v[2] = {0.0f, 0.0f};
                 if (tok < tokens && r < rank) {
                     const float *h = a.h + (size_t)plan.s_list[tok] * width + a.hoff[i] + r;
@@ -455,41 +460,44 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                 v[1] = r + 1 < rank ? v[1] * scale : 0.0f;
                 uint32_t t[3];
                 split3(v[0], v[1], t[0], t[1], t[2]);
-                const uint32_t to = h_smem + q * 3 * kHTile + tok * 128 + (((e >> 2 & 7) ^ (tok & 7)) << 4) + (e & 3) * 4;
+                const uint32_t to = h_smem + q * kHTile + tok * 128 + (((e >> 2 & 7) ^ (tok & 7)) << 4) + (e & 3) * 4;
 #pragma unroll
-                for (int z = 0; z < 3; ++z) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + z * kHTile), "r"(t[z]) : "memory");
+                for (int z = 0; z < 3; ++z) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + z * rows_term * 128), "r"(t[z]) : "memory");
             }
             fence_proxy_async_smem();
             __syncthreads();
             if (warp == 9) {
                 // ---- mma
                 if (elect_one()) {
-                    const uint32_t idesc = idesc_tokens(tokens > 16 ? 32 : 16);
+                    const uint32_t idesc = idesc_cols(3 * rows_term);
                     bool alive = true;
                     for (int k = 0; k < n && chunks && alive; ++k) {
                         const int no = task_no + k;
                         if (no >= kAcc) alive = hold(acc_free(no), ((no / kAcc) - 1) & 1);
-                        const uint32_t d = tmem + (no & (kAcc - 1)) * kTokE;
+                        const uint32_t d = tmem + (no & (kAcc - 1)) * kAccCols;
                         for (int q = 0; q < chunks && alive; ++q) {
                             const int st = stage_of(k, q);
                             alive = fix && q == chunks - 1 ? hold(fixed(fixes + k), ((fixes + k) / kRing) & 1) : hold(full(st), (st / kRing) & 1);
                             if (!alive) break;
                             tc_fence_after();
-                            const uint32_t b_smem = ring + (st & (kRing - 1)) * kBlockB, hq = h_smem + q * 3 * kHTile;
+                            const uint64_t bd = desc_sw128(ring + (st & (kRing - 1)) * kBlockB), hd = desc_sw128(h_smem + q * kHTile);
                             const int steps = min(4, (rank - q * 64 + 15) / 16);
-                            for (int z = 0; z < 3; ++z)
-                                for (int s = 0; s < steps; ++s)
-                                    mma_f16_ss(d, desc_sw128(b_smem + s * 32), desc_sw128(hq + z * kHTile + s * 32), idesc, q || z || s);
+#pragma unroll
+                            for (int s = 0; s < 4; ++s)      // 16 ranks are 32 bytes further on
+                                if (s < steps) mma_f16_ss(d, bd + 2 * s, hd + 2 * s, idesc, q || s);
                             tc_commit(empty(st));
                         }
                         if (alive) tc_commit(acc_full(no));
                     }
                 }
                 __syncwarp();                        // the warp comes to the barriers below as one
-            } else if (warp == 10) {
+            } else if (warp == 8) {
+                if (elect_one()) load(kRing, n * chunks);
+                __syncwarp();
+            } else if (warp >= 10) {
                 // ---- fix
                 bool alive = true;
-                for (int k = 0; k < n && fix && alive; ++k) {
+                for (int k = warp - 10; k < n && fix && alive; k += kFixWarps) {
                     const int st = stage_of(k, chunks - 1), r0 = (rank & 63) & ~15;      // first rank of the last product, in its chunk
                     alive = __all_sync(0xffffffffu, hold(full(st), (st / kRing) & 1));
                     if (!alive) break;
@@ -512,31 +520,45 @@ __global__ void __launch_bounds__(kThreadsE, 1)
             } else if (warp < 8) {
                 // ---- epilogue
                 bool alive = true;
-                for (int k = warp >> 2; k < n && alive; k += 2) {
-                    const int no = task_no + k, col = (c + k) * kCols + (warp & 3) * 32 + lane;
-                    const bool live = col < M;
-                    float v[kTokE];
+                const int lane_col = (warp & 3) * 32 + lane;
+                auto load_base = [&](int k, float (&v)[kTokE]) {
+                    const int col = (c + k) * kCols + lane_col;
+                    const bool live = base && k < n && col < M;
 #pragma unroll
                     for (int t0 = 0; t0 < kTokE; t0 += 8) {
                         if (t0 < tokens) {
 #pragma unroll
-                            for (int t = t0; t < t0 + 8; ++t)
-                                v[t] = base && live && t < tokens ? base[(size_t)plan.s_list[t] * M + col] : 0.0f;
+                            for (int t = t0; t < t0 + 8; ++t) v[t] = live && t < tokens ? base[(size_t)plan.s_list[t] * M + col] : 0.0f;
                         }
                     }
+                };
+                float next[kTokE];                   // base of the team's next task: two tasks' loads are under way
+                load_base(warp >> 2, next);
+                for (int k = warp >> 2; k < n && alive; k += 2) {
+                    const int no = task_no + k, col = (c + k) * kCols + lane_col;
+                    const bool live = col < M;
+                    float v[kTokE];
+#pragma unroll
+                    for (int t = 0; t < kTokE; ++t) v[t] = next[t];
+                    load_base(k + 2, next);
                     if (chunks) {
                         alive = __all_sync(0xffffffffu, hold(acc_full(no), (no / kAcc) & 1));
                         if (!alive) break;
                         tc_fence_after();
-                        const uint32_t d = tmem + ((uint32_t)(warp & 3) << 21) + (no & (kAcc - 1)) * kTokE;
+                        const uint32_t d = tmem + ((uint32_t)(warp & 3) << 21) + (no & (kAcc - 1)) * kAccCols;
 #pragma unroll
-                        for (int t0 = 0; t0 < kTokE; t0 += 16) {
+                        for (int t0 = 0; t0 < kTokE; t0 += 8) {
                             if (t0 < tokens) {
-                                uint32_t w[16];
-                                tmem_ld16(d + t0, w);
-                                tmem_wait_ld16(w);
+                                uint32_t w0[8], w1[8], w2[8];
+                                tmem_ld8(d + t0, w0);
+                                tmem_ld8(d + rows_term + t0, w1);
+                                tmem_ld8(d + 2 * rows_term + t0, w2);
+                                tmem_wait_ld8(w0);
+                                tmem_wait_ld8(w1);
+                                tmem_wait_ld8(w2);
 #pragma unroll
-                                for (int t = 0; t < 16; ++t) v[t0 + t] += __uint_as_float(w[t]);
+                                for (int t = 0; t < 8; ++t)
+                                    v[t0 + t] += __uint_as_float(w0[t]) + (__uint_as_float(w1[t]) + __uint_as_float(w2[t]));
                             }
                         }
                         tc_fence_before();
@@ -581,7 +603,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
     }
     __syncthreads();
     tc_fence_after();
-    if (warp == 9) tmem_dealloc(tmem, kAcc * kTokE);
+    if (warp == 9) tmem_dealloc(tmem, kAcc * kAccCols);
 }
 
 float *g_h = nullptr;
@@ -660,7 +682,7 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
     if (blocks * tiles_e > 0x7fffffffll) return -3;
     const int chunks = (most + 63) / 64;
     const size_t shrink_smem = (size_t)kRingBytes + Plan<kTok>::bytes(a.adapters, piece);
-    const size_t expand_smem = 1024 + (size_t)kRing * kBlockB + (size_t)chunks * 3 * kHTile + Plan<kTokE>::bytes(a.adapters, piece);
+    const size_t expand_smem = 1024 + (size_t)kRing * kBlockB + (size_t)chunks * kHTile + Plan<kTokE>::bytes(a.adapters, piece);
     static bool set = false;
     if (!set) {
         TQ_CHECK(cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));

@@ -80,6 +80,8 @@ CASES = [
     ([320, 320], 5, 72, 2080, 130),
     ([1040], 3, 40, 640, 700),
     ([64, 32, 16, 48], 300, 8, 64, 200),
+    ([2560, 1296], 3, 72, 64, 3000),
+    ([1920], 30, 64, 96, 4500),
 ]
 
 
