@@ -349,20 +349,15 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                         tc_fence_after();
                         const float f = grows ? exp2_approx(m - mx) : 1.0f;
                         l *= f;
+                        // a short loop: unrolled, its registers push others of the block loop out
+#pragma unroll 1
+                        for (int x = 0; x < D; x += 16) {
+                            uint32_t v[16];
+                            tmem_ld16(o_col + x, v);
+                            tmem_wait_ld16(v);
 #pragma unroll
-                        for (int x = 0; x < D; x += 32) {
-                            uint32_t v[32];
-                            tmem_ld32(o_col + x, v);
-                            tmem_wait32(v);
-#pragma unroll
-                            for (int y = 0; y < 32; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) * f);
-                            uint32_t w[16];
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) w[y] = v[y];
-                            tmem_st16(o_col + x, w);
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) w[y] = v[16 + y];
-                            tmem_st16(o_col + x + 16, w);
+                            for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) * f);
+                            tmem_st16(o_col + x, v);
                         }
                     }
                     if (grows) m = mx;
