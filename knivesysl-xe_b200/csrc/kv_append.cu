@@ -24,6 +24,7 @@ namespace tq {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kBatch = 4;             // head rows of a warp whose loads are under way together
 
 struct AppendArgs {
     KvArgs kv;
@@ -35,7 +36,7 @@ struct AppendArgs {
     int rot, interleaved;
     const uint16_t *q_norm, *k_norm;
     float eps;
-    int rows_per_warp;           // head rows of a token that one warp takes in turn
+    int parts, rows_per_warp;    // warps that share a token, head rows that each takes in turn
 };
 
 // The request of token t: the last r with start[r] <= t, 32 candidates per step.
@@ -90,13 +91,29 @@ template <int D, bool E4M3>
 __global__ void __launch_bounds__(kWarps * 32) kv_append_kernel(const AppendArgs a) {
     constexpr int E = D / 32;
     const int lane = threadIdx.x & 31;
-    const int t = blockIdx.x;
+    const unsigned number = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int t = (int)(number / (unsigned)a.parts);
     const int rows = a.q_heads + 2 * a.kv.heads;
-    const int row0 = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * a.rows_per_warp;
+    const int row0 = (int)(number % (unsigned)a.parts) * a.rows_per_warp;
     const int row1 = min(rows, row0 + a.rows_per_warp);
     pdl_wait();
     pdl_trigger();
-    if (row0 >= rows) return;
+    if (t >= a.kv.tokens || row0 >= rows) return;
+    // the first rows' loads need only the token's number: they are under way while its request is looked up
+    const int e0 = lane * E;
+    auto source = [&](int row) -> const float * {
+        if (row < a.q_heads) return a.q + (size_t)t * a.ldq + (size_t)row * D + e0;
+        row -= a.q_heads;
+        if (row < a.kv.heads) return a.k + (size_t)t * a.ldk + (size_t)row * D + e0;
+        return a.v + (size_t)t * a.ldv + (size_t)(row - a.kv.heads) * D + e0;
+    };
+    float next[kBatch][E];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (first + i < row1) load_row<E>(source(first + i), next[i]);
+    };
+    load(row0);
     const int r = find_request(a.kv, t, lane);
     const KvRequest req = kv_request(a.kv, r);
     const int i = t - req.t0;
@@ -105,7 +122,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_append_kernel(const AppendArgs
 
     // this lane's cosines and sines, with the sign that the partner's product takes
     float cs[E], sn[E];
-    const int half = a.rot >> 1, e0 = lane * E;
+    const int half = a.rot >> 1;
     const bool turns = e0 < a.rot;                 // rot is a multiple of 16: whole lanes turn or not
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -120,64 +137,69 @@ __global__ void __launch_bounds__(kWarps * 32) kv_append_kernel(const AppendArgs
             if (!a.interleaved && e0 < half) sn[e] = -sn[e];
         }
     }
+    // 1 + w of this lane's values
+    float gq[E], gk[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        gq[e] = a.q_norm && row0 < a.q_heads ? 1.0f + __uint_as_float((uint32_t)__ldg(a.q_norm + e0 + e) << 16) : 1.0f;
+        gk[e] = a.k_norm && row1 > a.q_heads ? 1.0f + __uint_as_float((uint32_t)__ldg(a.k_norm + e0 + e) << 16) : 1.0f;
+    }
     const int partner = a.interleaved || !turns ? lane : (e0 < half ? lane + half / E : lane - half / E);
 
     // the cache slot, for the lanes' k and v rows (the head moves it by whole pages' rows)
     const long long slot = row1 > a.q_heads ? kv_row(a.kv, r, 0, pos) : -1;
 
-    float next[E];
-    auto source = [&](int row) -> const float * {
-        if (row < a.q_heads) return a.q + (size_t)t * a.ldq + (size_t)row * D;
-        row -= a.q_heads;
-        if (row < a.kv.heads) return a.k + (size_t)t * a.ldk + (size_t)row * D;
-        return a.v + (size_t)t * a.ldv + (size_t)(row - a.kv.heads) * D;
-    };
-    load_row<E>(source(row0) + e0, next);
-    for (int row = row0; row < row1; ++row) {
-        float x[E];
+    for (int first = row0; first < row1; first += kBatch) {
+        float rowv[kBatch][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = next[e];
-        if (row + 1 < row1) load_row<E>(source(row + 1) + e0, next);
-        const bool is_q = row < a.q_heads, is_v = row >= a.q_heads + a.kv.heads;
-        if (!is_v) {
-            const uint16_t *w = is_q ? a.q_norm : a.k_norm;
-            if (w) {
-                float ss = 0.0f;
+        for (int i = 0; i < kBatch; ++i)
 #pragma unroll
-                for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
+                for (int e = 0; e < E; ++e) rowv[i][e] = next[i][e];
+        if (first + kBatch < row1) load(first + kBatch);
 #pragma unroll
-                for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-                const float f = __frsqrt_rn(ss * (1.0f / D) + a.eps);
+        for (int b = 0; b < kBatch; ++b) {
+            const int row = first + b;
+            if (row >= row1) break;
+            float (&x)[E] = rowv[b];
+            const bool is_q = row < a.q_heads, is_v = row >= a.q_heads + a.kv.heads;
+            if (!is_v) {
+                if (is_q ? a.q_norm : a.k_norm) {
+                    float ss = 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    x[e] = x[e] * f * (1.0f + __uint_as_float((uint32_t)__ldg(w + e0 + e) << 16));
-            }
-            if (a.interleaved) {
-                if (turns)
+                    for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-                    for (int e = 0; e < E; e += 2) {
-                        const float u = x[e], v = x[e + 1];
-                        x[e] = fmaf(u, cs[e], -(v * sn[e]));
-                        x[e + 1] = fmaf(v, cs[e], u * sn[e]);
+                    for (int off = 16; off >= 1; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+                    const float f = __frsqrt_rn(ss * (1.0f / D) + a.eps);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] = x[e] * f * (is_q ? gq[e] : gk[e]);
+                }
+                if (a.interleaved) {
+                    if (turns)
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) {
+                            const float u = x[e], v = x[e + 1];
+                            x[e] = fmaf(u, cs[e], -(v * sn[e]));
+                            x[e + 1] = fmaf(v, cs[e], u * sn[e]);
+                        }
+                } else if (a.rot) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float o = __shfl_sync(0xffffffffu, x[e], partner);
+                        if (turns) x[e] = fmaf(x[e], cs[e], o * sn[e]);
                     }
-            } else if (a.rot) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float o = __shfl_sync(0xffffffffu, x[e], partner);
-                    if (turns) x[e] = fmaf(x[e], cs[e], o * sn[e]);
                 }
             }
+            if (is_q) {
+                if (a.q_out) store_bf16<E>(a.q_out + ((size_t)t * a.q_heads + row) * D + e0, x);
+                continue;
+            }
+            if (slot < 0) continue;
+            const int g = row - a.q_heads - (is_v ? a.kv.heads : 0);
+            const size_t at = ((size_t)slot + (size_t)g * a.kv.page_size) * D + e0;
+            uint8_t *pool = is_v ? a.kv.v : a.kv.k;
+            if constexpr (E4M3) store_e4m3<E>(pool + at, x, is_v ? a.kv.v_scale : a.kv.k_scale);
+            else store_bf16<E>(reinterpret_cast<uint16_t *>(pool) + at, x);
         }
-        if (is_q) {
-            if (a.q_out) store_bf16<E>(a.q_out + ((size_t)t * a.q_heads + row) * D + e0, x);
-            continue;
-        }
-        if (slot < 0) continue;
-        const int g = row - a.q_heads - (is_v ? a.kv.heads : 0);
-        const size_t at = ((size_t)slot + (size_t)g * a.kv.page_size) * D + e0;
-        uint8_t *pool = is_v ? a.kv.v : a.kv.k;
-        if constexpr (E4M3) store_e4m3<E>(pool + at, x, is_v ? a.kv.v_scale : a.kv.k_scale);
-        else store_bf16<E>(reinterpret_cast<uint16_t *>(pool) + at, x);
     }
 }
 
@@ -280,10 +302,14 @@ int x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq
     a.q_out = d_q_out;
     a.q_heads = q_heads;
     const int rows = q_heads + 2 * a.kv.heads;
-    a.rows_per_warp = (rows + kWarps - 1) / kWarps;
-    while (a.rows_per_warp > 1 && (long long)a.kv.tokens * ((rows + a.rows_per_warp * kWarps - 1) / (a.rows_per_warp * kWarps)) < 592)
-        a.rows_per_warp = (a.rows_per_warp + 1) / 2;
-    const dim3 grid(a.kv.tokens, (rows + a.rows_per_warp * kWarps - 1) / (a.rows_per_warp * kWarps));
+    // As few warps a token as fill the GPU (32 an SM): the request, its page and the angles are looked up once a warp,
+    // which costs as much as some ten head rows. 2156 tokens of 56 rows: 28 us with 8 warps a token.
+    const long long want = 32ll * 148;
+    a.parts = (int)std::min<long long>(rows, (want + a.kv.tokens - 1) / a.kv.tokens);
+    a.rows_per_warp = (rows + a.parts - 1) / a.parts;
+    const long long warps = (long long)a.kv.tokens * a.parts;
+    if (warps > 0x7fffffffll) return -3;
+    const dim3 grid((unsigned)((warps + kWarps - 1) / kWarps));
     if (D == 64) launch<64>(a, cache->e4m3 != 0, grid);
     else if (D == 128) launch<128>(a, cache->e4m3 != 0, grid);
     else launch<256>(a, cache->e4m3 != 0, grid);

@@ -317,8 +317,8 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
 //   mma       one thread: 4 products per 64 ranks, h's three terms beside one another as columns
 //   fix       for a rank that ends inside 16: zeros over what lies beyond it in the last product (whatever B holds
 //             there must not get in). About a microsecond a task, mostly latency: four warps take tasks in turn
-//   epilogue  two teams of four warps, which take turns at the tasks, the base rows of the team's next task
-//             under way meanwhile
+//   epilogue  three teams of four warps, which take turns at the tasks: a team's base rows are under way before it
+//             waits for the product, and the other teams' meanwhile
 // h of the tile, scaled and split into its terms, lies in shared memory as [64 ranks][term][token], rows of
 // 128 bytes with the 128-byte swizzle, as B does. Up to 16 tokens it has 16 rows a term, else 32.
 constexpr int kCols = 128;
@@ -327,7 +327,9 @@ constexpr int kHTile = 3 * kTokE * 128;           // 64 ranks of h, its three te
 constexpr int kAcc = 4;                           // accumulators in tensor memory, of a column per term and token
 constexpr int kAccCols = 128;
 constexpr int kFixWarps = 4;
-constexpr int kThreadsE = (10 + kFixWarps) * 32;  // 8 warps epilogue, load, mma, fix
+constexpr int kTeams = 3;                         // of four warps, in the epilogue
+constexpr int kLoadWarp = 4 * kTeams, kMmaWarp = kLoadWarp + 1, kFixWarp = kMmaWarp + 1;
+constexpr int kThreadsE = (kFixWarp + kFixWarps) * 32;
 
 struct LoraMaps {
     CUtensorMap b[4];                             // B as rows [adapter x M] of rank values
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
         mbar_init_fence();
         s_gave_up = 0;
     }
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         tmem_alloc(smem_u32(&s_tmem), kAcc * kAccCols);
         tmem_relinquish();
         tc_fence_before();
@@ -430,7 +432,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                     tma_load_2d(ring + (st & (kRing - 1)) * kBlockB, &maps.b[i], q * 64, id * M + (c + k) * kCols, full(st));
                 }
             };
-            if (warp == 8) {
+            if (warp == kLoadWarp) {
                 if (elect_one()) load(0, min(n * chunks, kRing));
                 __syncwarp();
             }
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
             }
             fence_proxy_async_smem();
             __syncthreads();
-            if (warp == 9) {
+            if (warp == kMmaWarp) {
                 // ---- mma
                 if (elect_one()) {
                     const uint32_t idesc = idesc_cols(3 * rows_term);
@@ -491,13 +493,13 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                     }
                 }
                 __syncwarp();                        // the warp comes to the barriers below as one
-            } else if (warp == 8) {
+            } else if (warp == kLoadWarp) {
                 if (elect_one()) load(kRing, n * chunks);
                 __syncwarp();
-            } else if (warp >= 10) {
+            } else if (warp >= kFixWarp) {
                 // ---- fix
                 bool alive = true;
-                for (int k = warp - 10; k < n && fix && alive; k += kFixWarps) {
+                for (int k = warp - kFixWarp; k < n && fix && alive; k += kFixWarps) {
                     const int st = stage_of(k, chunks - 1), r0 = (rank & 63) & ~15;      // first rank of the last product, in its chunk
                     alive = __all_sync(0xffffffffu, hold(full(st), (st / kRing) & 1));
                     if (!alive) break;
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(fixed(fixes + k));
                 }
-            } else if (warp < 8) {
+            } else {
                 // ---- epilogue
                 bool alive = true;
                 const int lane_col = (warp & 3) * 32 + lane;
@@ -532,15 +534,11 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                         }
                     }
                 };
-                float next[kTokE];                   // base of the team's next task: two tasks' loads are under way
-                load_base(warp >> 2, next);
-                for (int k = warp >> 2; k < n && alive; k += 2) {
+                for (int k = warp >> 2; k < n && alive; k += kTeams) {
                     const int no = task_no + k, col = (c + k) * kCols + lane_col;
                     const bool live = col < M;
                     float v[kTokE];
-#pragma unroll
-                    for (int t = 0; t < kTokE; ++t) v[t] = next[t];
-                    load_base(k + 2, next);
+                    load_base(k, v);
                     if (chunks) {
                         alive = __all_sync(0xffffffffu, hold(acc_full(no), (no / kAcc) & 1));
                         if (!alive) break;
@@ -592,9 +590,9 @@ __global__ void __launch_bounds__(kThreadsE, 1)
     }
     if (!waited) pdl_wait();
     __syncthreads();
-    if (warp == 8 && s_gave_up && lane == 0)         // copies may still be under way: they end before the CTA does
+    if (warp == kLoadWarp && s_gave_up && lane == 0)         // copies may still be under way: they end before the CTA does
         for (int st = max(0, at - kRing); st < at; ++st) mbar_wait_bounded(full(st), (st / kRing) & 1, a.status, 25, limit_ns);
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         if (elect_one()) {
             tc_commit(drained);
             mbar_wait_bounded(drained, 0, a.status, 25, limit_ns);
@@ -603,7 +601,7 @@ __global__ void __launch_bounds__(kThreadsE, 1)
     }
     __syncthreads();
     tc_fence_after();
-    if (warp == 9) tmem_dealloc(tmem, kAcc * kAccCols);
+    if (warp == kMmaWarp) tmem_dealloc(tmem, kAcc * kAccCols);
 }
 
 float *g_h = nullptr;
