@@ -43,7 +43,11 @@ constexpr int kCubic = 2;             // of four pairs of exponentials, those th
 template <int D, Load LOAD, int TERMS>
 struct TileShape {
     static constexpr int kLoadWarps = LOAD == kTma ? 1 : 4;
-    static constexpr int kTiles = D <= 128 ? 2 : 1;                 // row tiles of a CTA
+    // Three terms of P: the second and third add to sums of their own, where tensor memory has room for them beside one
+    // row tile. The tensor core cuts an fp32 sum off instead of rounding it, 12 times per 64 keys in one sum for all
+    // terms, 4 times in the first term's own (4000 keys: off by 2e-6 of a row with one sum).
+    static constexpr bool kLow = TERMS == 3 && D <= 128;
+    static constexpr int kTiles = D <= 128 && !kLow ? 2 : 1;        // row tiles of a CTA
     static constexpr int kRows = kRowsTile * kTiles;
     static constexpr int kKeys = 64;                                // of a block
     // Score buffers of a tile. With two, the scores of block j + 1 lie ready when the probabilities of
@@ -173,7 +177,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
     constexpr int kT = S::kTiles, kN = S::kKeys;
     constexpr bool OUT_BF16 = TERMS == 1;
     constexpr int kBuf = S::kBuf, kScores = kT * kBuf;
-    constexpr uint32_t kSlotCol = 256;                 // tensor memory: O tiles, then the slots of S and P
+    constexpr uint32_t kSlotCol = 256;                 // tensor memory: O tiles (and the lower terms' sums), then the slots of S and P
     constexpr uint32_t kQkDesc = idesc_f16(128, kN, !E4M3, false), kPvDesc = idesc_f16(128, D, !E4M3, true);
 
     extern __shared__ uint8_t smem_raw[];
@@ -351,7 +355,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                         l *= f;
                         // a short loop: unrolled, its registers push others of the block loop out
 #pragma unroll 1
-                        for (int x = 0; x < D; x += 16) {
+                        for (int x = 0; x < (S::kLow ? 2 * D : D); x += 16) {
                             uint32_t v[16];
                             tmem_ld16(o_col + x, v);
                             tmem_wait_ld16(v);
@@ -408,6 +412,17 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 tc_fence_after();
             }
             // ---- the tile's rows, or this CTA's part of them
+            auto load_o = [&](int x, uint32_t (&v)[32]) {
+                tmem_ld32(o_col + x, v);
+                tmem_wait32(v);
+                if constexpr (S::kLow) {
+                    uint32_t w[32];
+                    tmem_ld32(o_col + D + x, w);
+                    tmem_wait32(w);
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) + __uint_as_float(w[y]));
+                }
+            };
             const bool whole = first == 0 && last == line.units;
             if (whole) {
                 const float f = l > 0.0f ? __fdiv_rn(a.kv.v_scale, l) : (l == l ? 0.0f : l);
@@ -416,8 +431,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
 #pragma unroll
                     for (int x = 0; x < D; x += 32) {
                         uint32_t v[32];
-                        tmem_ld32(o_col + x, v);
-                        tmem_wait32(v);
+                        load_o(x, v);
                         if (!live) {
                         } else if constexpr (OUT_BF16) {
                             uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to + x);
@@ -446,8 +460,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
 #pragma unroll
                     for (int x = 0; x < D; x += 32) {
                         uint32_t v[32];
-                        tmem_ld32(o_col + x, v);
-                        tmem_wait32(v);
+                        load_o(x, v);
 #pragma unroll
                         for (int y = 0; y < 32; ++y) part[(x + y) * kRowsTile] = __uint_as_float(v[y]);
                     }
@@ -624,8 +637,8 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 for (int z = 0; z < TERMS; ++z)
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
-                        mma_f16_ts(d, p + (z ? 32 + 32 * z : 0) + k * 8, desc_of(vd + (k * 2048 >> 4)), kPvDesc,
-                                   z || k ? 1u : (fresh ? 0u : 1u));
+                        mma_f16_ts(S::kLow && z ? d + D : d, p + (z ? 32 + 32 * z : 0) + k * 8, desc_of(vd + (k * 2048 >> 4)), kPvDesc,
+                                   k || z > (S::kLow ? 1 : 0) ? 1u : (fresh ? 0u : 1u));
                 tc_commit(o_done(t));
                 if (closes) tc_commit(o_last(t));
             };
