@@ -6,7 +6,9 @@
 // of them (one for dim 256), each with its own scores S and sums O in tensor memory, so that the
 // tensor core multiplies for one while the other's probabilities are computed. Roles:
 //   softmax  one warpgroup per tile, a thread per row: its queries into shared memory, then per block
-//            of keys S -> running maximum -> P, written over S as the next product's A operand
+//            of keys S -> running maximum -> P, written over S as the next product's A operand. Where a
+//            CTA has one tile, two warpgroups take turns at its blocks; the maximum passes from one to the
+//            other through shared memory, the sums are added at the end
 //   load     the blocks of keys and values, page by page, into a ring in shared memory: one warp that
 //            issues TMA copies of 8 to 64 rows, or, where pages are no multiple of 8 or the cache is
 //            e4m3 (which becomes fp16 on the way), four warps through their registers
@@ -58,7 +60,7 @@ struct TileShape {
     static constexpr int kRing = 131072 / kBlock > 8 ? 8 : 131072 / kBlock;
     static constexpr int kQ = kRowsTile * D * 2;                    // bytes of a tile's queries
     static constexpr int kSmem = kTiles * kQ + kRing * kBlock + 1024;
-    static constexpr int kSoftmax = kTiles * 128;                   // threads
+    static constexpr int kSoftmax = 256;                            // threads: a warpgroup per tile, or two that share one
     static constexpr int kThreads = kSoftmax + kLoadWarps * 32 + kTiles * 32;
 };
 
@@ -182,9 +184,10 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ long long s_scan[S::kThreads / 32 + 3];
-    __shared__ __align__(8) uint64_t s_bar[2 * S::kRing + 2 * kScores + 3 * kT + 2];
+    __shared__ __align__(8) uint64_t s_bar[2 * S::kRing + 2 * kScores + 3 * kT + 3];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_gave_up;
+    __shared__ float s_c[128], s_m[128], s_ml[2][2][128];        // one tile: factor, maximum of each row; (m, l) of each warpgroup
+    __shared__ int s_gave_up, s_stop;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
     const int G = a.group;
@@ -200,11 +203,13 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
     auto o_last = [&](int i) { return bars + 8 * (2 * S::kRing + 2 * kScores + 2 * kT + i); };   // the last one of a stretch's tile
     const uint32_t drained = bars + 8 * (2 * S::kRing + 2 * kScores + 3 * kT);       // all products and their arrivals are done
 
+    const uint32_t m_ready = drained + 16;             // one tile: the maximum up to a block is in s_m
     const uint32_t landed = drained + 8;               // a block that the load warp has to complete itself
 
     if (tid == 0) {
         mbar_init(drained, kT);
         mbar_init(landed, 1);
+        mbar_init(m_ready, 4);
         for (int i = 0; i < S::kRing; ++i) {
             mbar_init(full(i), S::kLoadWarps);
             mbar_init(empty(i), kT);
@@ -214,7 +219,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
             mbar_init(p_full(i), 4);
         }
         for (int i = 0; i < kT; ++i) {
-            mbar_init(q_full(i), 4);
+            mbar_init(q_full(i), S::kSoftmax / 32 / kT);
             mbar_init(o_done(i), 1);
             mbar_init(o_last(i), 1);
         }
@@ -252,12 +257,13 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
 
     if (warp < S::kSoftmax / 32) {
         // ================================ softmax ================================================
-        const int t = warp >> 2, row = tid & 127;
+        constexpr int kGroups = 2 / kT;                    // warpgroups of a tile
+        const int t = kT == 2 ? warp >> 2 : 0, wg = kT == 2 ? 0 : warp >> 2, row = tid & 127;
         const uint32_t lane_col = tmem + ((uint32_t)(warp & 3) << 21);
         const uint32_t o_col = lane_col + t * D;
-        uint32_t s_phase = 0, o_count = 0, tiles_done = 0;   // a bit per slot; products of this tile; tiles
-        bool alive = true;
-        for (long long u = line.begin; alive;) {
+        uint32_t s_phase = 0, blocks_done = 0, tiles_done = 0;     // a bit per slot; blocks and tiles of this tile so far
+        bool alive = true;                                 // no wait of this warp gave up
+        for (long long u = line.begin;;) {
             const KvRequest req = line.q;
             const int first = line.first_unit(u), last = line.last_unit();
             if (last <= first) break;
@@ -273,17 +279,18 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 const long long mine = live ? ((long long)(req.t0 + tok) * a.q_heads + line.g * G + rho % G) * D : -1;
                 const uint32_t q_tile = q_smem + t * S::kQ;
                 constexpr int kQChunks = D / 8;            // 16-byte chunks of a row
-                uint4 v[8];
+                constexpr int kShare = kQChunks / kGroups, kAtOnce = kShare < 8 ? kShare : 8;
+                uint4 v[kAtOnce];
 #pragma unroll
-                for (int x0 = 0; x0 < kQChunks; x0 += 8) {
+                for (int x0 = wg * kShare; x0 < (wg + 1) * kShare; x0 += kAtOnce) {
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {
+                    for (int x = 0; x < kAtOnce; ++x) {
                         const int i = (x0 + x) * 32 + lane;
                         const long long from = __shfl_sync(0xffffffffu, mine, i / kQChunks);
                         v[x] = from >= 0 ? __ldg(reinterpret_cast<const uint4 *>(a.q + from) + i % kQChunks) : make_uint4(0, 0, 0, 0);
                     }
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {
+                    for (int x = 0; x < kAtOnce; ++x) {
                         const int i = (x0 + x) * 32 + lane, r = (warp & 3) * 32 + i / kQChunks, ch = i % kQChunks;
                         st_shared16(q_tile + (ch >> 3) * (kRowsTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
                                     make_uint4((v[x].x ^ flip) & keep, (v[x].y ^ flip) & keep, (v[x].z ^ flip) & keep,
@@ -292,23 +299,31 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 }
                 if constexpr (E4M3) {
                     // own row: to fp16, times the power of two that takes its largest value to [2^9, 2^10)
-                    __syncwarp();
-                    auto place = [&](int ch) { return q_tile + (ch >> 3) * (kRowsTile * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
-                    uint32_t top = 0;
+                    if constexpr (kGroups == 2) named_bar_sync(2, 256);
+                    else __syncwarp();
+                    if (wg == 0) {
+                        auto place = [&](int ch) { return q_tile + (ch >> 3) * (kRowsTile * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
+                        uint32_t top = 0;
 #pragma unroll 8
-                    for (int ch = 0; ch < kQChunks; ++ch) {
-                        const uint4 w = ld_shared16(place(ch));
-                        top = max(max(top, max(w.x << 16 & 0x7fff0000u, w.x & 0x7fff0000u)), max(w.y << 16 & 0x7fff0000u, w.y & 0x7fff0000u));
-                        top = max(max(top, max(w.z << 16 & 0x7fff0000u, w.z & 0x7fff0000u)), max(w.w << 16 & 0x7fff0000u, w.w & 0x7fff0000u));
+                        for (int ch = 0; ch < kQChunks; ++ch) {
+                            const uint4 w = ld_shared16(place(ch));
+                            top = max(max(top, max(w.x << 16 & 0x7fff0000u, w.x & 0x7fff0000u)), max(w.y << 16 & 0x7fff0000u, w.y & 0x7fff0000u));
+                            top = max(max(top, max(w.z << 16 & 0x7fff0000u, w.z & 0x7fff0000u)), max(w.w << 16 & 0x7fff0000u, w.w & 0x7fff0000u));
+                        }
+                        const int ex = min(max((int)(top >> 23) - 127, -100), 127);
+                        const float by = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
+                        c *= __uint_as_float((uint32_t)(127 - 9 + ex) << 23);
+#pragma unroll 8
+                        for (int ch = 0; ch < kQChunks; ++ch) {
+                            const uint4 w = ld_shared16(place(ch));
+                            st_shared16(place(ch), make_uint4(pack_f16(bf16_lo(w.x) * by, bf16_hi(w.x) * by), pack_f16(bf16_lo(w.y) * by, bf16_hi(w.y) * by),
+                                                              pack_f16(bf16_lo(w.z) * by, bf16_hi(w.z) * by), pack_f16(bf16_lo(w.w) * by, bf16_hi(w.w) * by)));
+                        }
+                        s_c[row] = c;
                     }
-                    const int ex = min(max((int)(top >> 23) - 127, -100), 127);
-                    const float by = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
-                    c *= __uint_as_float((uint32_t)(127 - 9 + ex) << 23);
-#pragma unroll 8
-                    for (int ch = 0; ch < kQChunks; ++ch) {
-                        const uint4 w = ld_shared16(place(ch));
-                        st_shared16(place(ch), make_uint4(pack_f16(bf16_lo(w.x) * by, bf16_hi(w.x) * by), pack_f16(bf16_lo(w.y) * by, bf16_hi(w.y) * by),
-                                                          pack_f16(bf16_lo(w.z) * by, bf16_hi(w.z) * by), pack_f16(bf16_lo(w.w) * by, bf16_hi(w.w) * by)));
+                    if constexpr (kGroups == 2) {
+                        named_bar_sync(2, 256);
+                        c = s_c[row];
                     }
                 }
                 if (!(c > 0.0f)) c = 1.17549435e-38f;      // scores of no size: any factor above 0
@@ -316,7 +331,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full(t));
 
-                for (int j = first; j < end; ++j) {
+                for (int j = first + wg; j < end && alive; j += kGroups) {
                     const int slot = t * kBuf + (kBuf == 2 ? (j - first) & 1 : 0);
                     const uint32_t s_col = lane_col + kSlotCol + slot * S::kSlotCols;
                     if (!wait(s_full(slot), s_phase >> slot & 1)) { alive = false; break; }
@@ -345,14 +360,28 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                     }
                     mx = fmaxf(mx, mx1);
                     mx *= c;
-                    const bool grows = mx > m + 8.0f;
+                    const uint32_t done = blocks_done + (j - first);       // blocks before this one
+                    float before = m;                      // the maximum that O and the blocks before have
+                    if constexpr (kGroups == 2) {
+                        before = -INFINITY;
+                        if (j > first) {
+                            if (!wait(m_ready, (done - 1) & 1)) { alive = false; break; }
+                            before = s_m[row];
+                        }
+                    }
+                    const bool grows = mx > before + 8.0f;
+                    const float now = grows ? mx : before;
+                    if constexpr (kGroups == 2) {
+                        s_m[row] = now;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(m_ready);
+                    }
                     if (j > first && __any_sync(0xffffffffu, grows)) {
                         // The product of block j - 1 must be in O. That of j - 2 is (the scores of block j were
                         // multiplied behind it), so the barrier is at most one phase behind.
-                        if (!wait(o_done(t), (o_count - 1) & 1)) { alive = false; break; }
+                        if (!wait(o_done(t), (done - 1) & 1)) { alive = false; break; }
                         tc_fence_after();
-                        const float f = grows ? exp2_approx(m - mx) : 1.0f;
-                        l *= f;
+                        const float f = grows ? exp2_approx(before - mx) : 1.0f;
                         // a short loop: unrolled, its registers push others of the block loop out
 #pragma unroll 1
                         for (int x = 0; x < (S::kLow ? 2 * D : D); x += 16) {
@@ -364,7 +393,11 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                             tmem_st16(o_col + x, v);
                         }
                     }
-                    if (grows) m = mx;
+                    // this thread's sum so far has the maximum that it last saw
+                    if (now != m) {
+                        l *= exp2_approx(m - now);
+                        m = now;
+                    }
                     const float off = m == -INFINITY ? 0.0f : -m;
                     // ---- probabilities, over the scores
                     f32x2 sum = pack2(0.0f, 0.0f);
@@ -406,12 +439,20 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(p_full(slot));
-                    ++o_count;
                 }
-                if (!alive || !wait(o_last(t), tiles_done++ & 1)) break;
+                blocks_done += end - first;
+                alive = alive && wait(o_last(t), tiles_done++ & 1);
                 tc_fence_after();
+                if constexpr (kGroups == 2) {
+                    s_ml[wg][0][row] = m;
+                    s_ml[wg][1][row] = l;
+                    named_bar_sync(2, 256);
+                    const float mo = s_ml[wg ^ 1][0][row], lo = s_ml[wg ^ 1][1][row], both = fmaxf(m, mo);
+                    if (both != -INFINITY) l = (m == -INFINITY ? 0.0f : l * exp2_approx(m - both)) + (mo == -INFINITY ? 0.0f : lo * exp2_approx(mo - both));
+                    m = both;
+                }
             }
-            // ---- the tile's rows, or this CTA's part of them
+            // ---- the tile's rows, or this CTA's part of them (whatever they hold, if a wait gave up)
             auto load_o = [&](int x, uint32_t (&v)[32]) {
                 tmem_ld32(o_col + x, v);
                 tmem_wait32(v);
@@ -429,7 +470,8 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 const size_t to = (size_t)(req.t0 + tok) * a.ldo + (size_t)(line.g * G + rho % G) * D;
                 if (first < end)
 #pragma unroll
-                    for (int x = 0; x < D; x += 32) {
+                    for (int xx = 0; xx < D / kGroups; xx += 32) {
+                        const int x = wg * (D / kGroups) + xx;
                         uint32_t v[32];
                         load_o(x, v);
                         if (!live) {
@@ -458,16 +500,27 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 float *part = a.part + (size_t)(slot * kT + t) * (D + 2) * kRowsTile + row;
                 if (first < end)
 #pragma unroll
-                    for (int x = 0; x < D; x += 32) {
+                    for (int xx = 0; xx < D / kGroups; xx += 32) {
+                        const int x = wg * (D / kGroups) + xx;
                         uint32_t v[32];
                         load_o(x, v);
 #pragma unroll
                         for (int y = 0; y < 32; ++y) part[(x + y) * kRowsTile] = __uint_as_float(v[y]);
                     }
-                part[D * kRowsTile] = m;
-                part[(D + 1) * kRowsTile] = l;
+                if (wg == 0) {
+                    part[D * kRowsTile] = m;
+                    part[(D + 1) * kRowsTile] = l;
+                }
             }
             tc_fence_before();
+            if constexpr (kGroups == 2) {
+                // O has been read by both, and both go on or end together: neither leaves the other at a barrier
+                if (tid == 0) s_stop = s_gave_up;
+                named_bar_sync(2, 256);
+                if (s_stop) break;
+            } else if (!alive) {
+                break;
+            }
             if (tid == 0 && first == 0 && last < line.units)      // the tile starts here and goes on: its parts
                 joins[cta] = JoinTile{req.t0, req.n, line.g, line.m, cta, line.cta_of(line.behind() - 1),
                                       2 * cta + (u == line.begin ? 0 : 1), 1};
