@@ -263,74 +263,113 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
         const uint32_t o_col = lane_col + t * D;
         uint32_t s_phase = 0, blocks_done = 0, tiles_done = 0;     // a bit per slot; blocks and tiles of this tile so far
         bool alive = true;                                 // no wait of this warp gave up
-        for (long long u = line.begin;;) {
-            const KvRequest req = line.q;
-            const int first = line.first_unit(u), last = line.last_unit();
-            if (last <= first) break;
-            const int end = tile_end(t, last), rows = tile_rows(t);
+        // A stretch's tile as this thread sees it.
+        struct Part {
+            int first, last, end;                          // units, and the end of this row tile's own
+            int limit, low;                                // last key that the row sees, that every row sees
+            bool live, whole;
+            long long query;                               // the row's place in q, -1 for none
+            size_t to;                                     // and in the output
+            float *part;                                   // where the tile is cut: its place in the parts
+            long long behind;
+        };
+        auto describe = [&](long long u) {
+            Part x;
+            const KvRequest &req = line.q;
+            x.first = line.first_unit(u);
+            x.last = line.last_unit();
+            x.end = tile_end(t, x.last);
             const int rho = line.m * S::kRows + t * kRowsTile + row, tok = rho / G;
-            const bool live = row < rows;
-            const int limit = live ? req.total - req.n + tok : -1;
-            const int low = req.total - req.n + (line.m * S::kRows + t * kRowsTile) / G;   // seen by all rows
-            float c = fabsf(a.c), m = -INFINITY, l = 0.0f;
+            x.live = row < tile_rows(t);
+            x.limit = x.live ? req.total - req.n + tok : -1;
+            x.low = req.total - req.n + (line.m * S::kRows + t * kRowsTile) / G;
+            x.whole = x.first == 0 && x.last == line.units;
+            x.query = x.live ? ((long long)(req.t0 + tok) * a.q_heads + line.g * G + rho % G) * D : -1;
+            x.to = (size_t)(req.t0 + tok) * a.ldo + (size_t)(line.g * G + rho % G) * D;
+            const int slot = 2 * cta + (u == line.begin ? 0 : 1);
+            x.part = a.part + (size_t)(slot * kT + t) * (D + 2) * kRowsTile + row;
+            x.behind = line.behind();
+            if (tid == 0 && x.first == 0 && x.last > 0 && !x.whole)      // the tile starts here and goes on: its parts
+                joins[cta] = JoinTile{req.t0, req.n, line.g, line.m, cta, line.cta_of(x.behind - 1), slot, 1};
+            return x;
+        };
+        // The queries of a tile into shared memory, once the products with the last ones are complete; the factor
+        // of the row's scores.
+        auto load_q = [&](const Part &x) {
+            float c = fabsf(a.c);
+            // ---- the warp's 32 rows of queries, turned by the sign of the scale, whole rows per load
+            const uint32_t flip = a.c < 0.0f ? 0x80008000u : 0u, keep = a.c != 0.0f ? 0xffffffffu : 0u;
+            const uint32_t q_tile = q_smem + t * S::kQ;
+            constexpr int kQChunks = D / 8;            // 16-byte chunks of a row
+            constexpr int kShare = kQChunks / kGroups, kAtOnce = kShare < 8 ? kShare : 8;
+            uint4 v[kAtOnce];
+#pragma unroll
+            for (int x0 = wg * kShare; x0 < (wg + 1) * kShare; x0 += kAtOnce) {
+#pragma unroll
+                for (int n = 0; n < kAtOnce; ++n) {
+                    const int i = (x0 + n) * 32 + lane;
+                    const long long from = __shfl_sync(0xffffffffu, x.query, i / kQChunks);
+                    v[n] = from >= 0 ? __ldg(reinterpret_cast<const uint4 *>(a.q + from) + i % kQChunks) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int n = 0; n < kAtOnce; ++n) {
+                    const int i = (x0 + n) * 32 + lane, r = (warp & 3) * 32 + i / kQChunks, ch = i % kQChunks;
+                    st_shared16(q_tile + (ch >> 3) * (kRowsTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                                make_uint4((v[n].x ^ flip) & keep, (v[n].y ^ flip) & keep, (v[n].z ^ flip) & keep,
+                                           (v[n].w ^ flip) & keep));
+                }
+            }
+            if constexpr (E4M3) {
+                // own row: to fp16, times the power of two that takes its largest value to [2^9, 2^10)
+                if constexpr (kGroups == 2) named_bar_sync(2, 256);
+                else __syncwarp();
+                if (wg == 0) {
+                    auto place = [&](int ch) { return q_tile + (ch >> 3) * (kRowsTile * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
+                    uint32_t top = 0;
+#pragma unroll 8
+                    for (int ch = 0; ch < kQChunks; ++ch) {
+                        const uint4 w = ld_shared16(place(ch));
+                        top = max(max(top, max(w.x << 16 & 0x7fff0000u, w.x & 0x7fff0000u)), max(w.y << 16 & 0x7fff0000u, w.y & 0x7fff0000u));
+                        top = max(max(top, max(w.z << 16 & 0x7fff0000u, w.z & 0x7fff0000u)), max(w.w << 16 & 0x7fff0000u, w.w & 0x7fff0000u));
+                    }
+                    const int ex = min(max((int)(top >> 23) - 127, -100), 127);
+                    const float by = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
+                    c *= __uint_as_float((uint32_t)(127 - 9 + ex) << 23);
+#pragma unroll 8
+                    for (int ch = 0; ch < kQChunks; ++ch) {
+                        const uint4 w = ld_shared16(place(ch));
+                        st_shared16(place(ch), make_uint4(pack_f16(bf16_lo(w.x) * by, bf16_hi(w.x) * by), pack_f16(bf16_lo(w.y) * by, bf16_hi(w.y) * by),
+                                                          pack_f16(bf16_lo(w.z) * by, bf16_hi(w.z) * by), pack_f16(bf16_lo(w.w) * by, bf16_hi(w.w) * by)));
+                    }
+                    s_c[row] = c;
+                }
+                if constexpr (kGroups == 2) {
+                    named_bar_sync(2, 256);
+                    c = s_c[row];
+                }
+            }
+            if (!(c > 0.0f)) c = 1.17549435e-38f;      // scores of no size: any factor above 0
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full(t));
+            return c;
+        };
+        Part cur = describe(line.begin);
+        if (cur.last <= cur.first) cur.end = 0;            // the stretch ends before the tile's first unit
+        float c = cur.first < cur.end ? load_q(cur) : 0.0f;
+        while (cur.last > cur.first) {
+            const int first = cur.first, end = cur.end, limit = cur.limit, low = cur.low;
+            const bool more = cur.behind < line.end, live = cur.live;
+            float m = -INFINITY, l = 0.0f, c_next = 0.0f;
+            Part next = cur;
+            next.last = next.first;                        // none
+            auto prepare = [&]() {                         // the stretch's next tile: its queries are on their way under this one's end
+                if (!more) return;
+                line.next();
+                next = describe(cur.behind);
+                if (next.last > next.first && next.first < next.end) c_next = load_q(next);
+            };
             if (first < end) {
-                // ---- the warp's 32 rows of queries, turned by the sign of the scale, whole rows per load
-                const uint32_t flip = a.c < 0.0f ? 0x80008000u : 0u, keep = a.c != 0.0f ? 0xffffffffu : 0u;
-                const long long mine = live ? ((long long)(req.t0 + tok) * a.q_heads + line.g * G + rho % G) * D : -1;
-                const uint32_t q_tile = q_smem + t * S::kQ;
-                constexpr int kQChunks = D / 8;            // 16-byte chunks of a row
-                constexpr int kShare = kQChunks / kGroups, kAtOnce = kShare < 8 ? kShare : 8;
-                uint4 v[kAtOnce];
-#pragma unroll
-                for (int x0 = wg * kShare; x0 < (wg + 1) * kShare; x0 += kAtOnce) {
-#pragma unroll
-                    for (int x = 0; x < kAtOnce; ++x) {
-                        const int i = (x0 + x) * 32 + lane;
-                        const long long from = __shfl_sync(0xffffffffu, mine, i / kQChunks);
-                        v[x] = from >= 0 ? __ldg(reinterpret_cast<const uint4 *>(a.q + from) + i % kQChunks) : make_uint4(0, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int x = 0; x < kAtOnce; ++x) {
-                        const int i = (x0 + x) * 32 + lane, r = (warp & 3) * 32 + i / kQChunks, ch = i % kQChunks;
-                        st_shared16(q_tile + (ch >> 3) * (kRowsTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
-                                    make_uint4((v[x].x ^ flip) & keep, (v[x].y ^ flip) & keep, (v[x].z ^ flip) & keep,
-                                               (v[x].w ^ flip) & keep));
-                    }
-                }
-                if constexpr (E4M3) {
-                    // own row: to fp16, times the power of two that takes its largest value to [2^9, 2^10)
-                    if constexpr (kGroups == 2) named_bar_sync(2, 256);
-                    else __syncwarp();
-                    if (wg == 0) {
-                        auto place = [&](int ch) { return q_tile + (ch >> 3) * (kRowsTile * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4); };
-                        uint32_t top = 0;
-#pragma unroll 8
-                        for (int ch = 0; ch < kQChunks; ++ch) {
-                            const uint4 w = ld_shared16(place(ch));
-                            top = max(max(top, max(w.x << 16 & 0x7fff0000u, w.x & 0x7fff0000u)), max(w.y << 16 & 0x7fff0000u, w.y & 0x7fff0000u));
-                            top = max(max(top, max(w.z << 16 & 0x7fff0000u, w.z & 0x7fff0000u)), max(w.w << 16 & 0x7fff0000u, w.w & 0x7fff0000u));
-                        }
-                        const int ex = min(max((int)(top >> 23) - 127, -100), 127);
-                        const float by = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
-                        c *= __uint_as_float((uint32_t)(127 - 9 + ex) << 23);
-#pragma unroll 8
-                        for (int ch = 0; ch < kQChunks; ++ch) {
-                            const uint4 w = ld_shared16(place(ch));
-                            st_shared16(place(ch), make_uint4(pack_f16(bf16_lo(w.x) * by, bf16_hi(w.x) * by), pack_f16(bf16_lo(w.y) * by, bf16_hi(w.y) * by),
-                                                              pack_f16(bf16_lo(w.z) * by, bf16_hi(w.z) * by), pack_f16(bf16_lo(w.w) * by, bf16_hi(w.w) * by)));
-                        }
-                        s_c[row] = c;
-                    }
-                    if constexpr (kGroups == 2) {
-                        named_bar_sync(2, 256);
-                        c = s_c[row];
-                    }
-                }
-                if (!(c > 0.0f)) c = 1.17549435e-38f;      // scores of no size: any factor above 0
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full(t));
-
                 for (int j = first + wg; j < end && alive; j += kGroups) {
                     const int slot = t * kBuf + (kBuf == 2 ? (j - first) & 1 : 0);
                     const uint32_t s_col = lane_col + kSlotCol + slot * S::kSlotCols;
@@ -441,6 +480,9 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                     if (lane == 0) mbar_arrive(p_full(slot));
                 }
                 blocks_done += end - first;
+                // With a tile of its own, a warpgroup has seen the scores of the last block: no product reads the
+                // queries any more. Of two, one may not have: there the last product is waited for first.
+                if constexpr (kGroups == 1) prepare();
                 alive = alive && wait(o_last(t), tiles_done++ & 1);
                 tc_fence_after();
                 if constexpr (kGroups == 2) {
@@ -450,7 +492,10 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                     const float mo = s_ml[wg ^ 1][0][row], lo = s_ml[wg ^ 1][1][row], both = fmaxf(m, mo);
                     if (both != -INFINITY) l = (m == -INFINITY ? 0.0f : l * exp2_approx(m - both)) + (mo == -INFINITY ? 0.0f : lo * exp2_approx(mo - both));
                     m = both;
+                    prepare();
                 }
+            } else {
+                prepare();
             }
             // ---- the tile's rows, or this CTA's part of them (whatever they hold, if a wait gave up)
             auto load_o = [&](int x, uint32_t (&v)[32]) {
@@ -464,10 +509,9 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                     for (int y = 0; y < 32; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) + __uint_as_float(w[y]));
                 }
             };
-            const bool whole = first == 0 && last == line.units;
-            if (whole) {
+            if (cur.whole) {
                 const float f = l > 0.0f ? __fdiv_rn(a.kv.v_scale, l) : (l == l ? 0.0f : l);
-                const size_t to = (size_t)(req.t0 + tok) * a.ldo + (size_t)(line.g * G + rho % G) * D;
+                const size_t to = cur.to;
                 if (first < end)
 #pragma unroll
                     for (int xx = 0; xx < D / kGroups; xx += 32) {
@@ -496,8 +540,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                     }
             } else {
                 // [dim][row]: neighbouring threads write neighbouring words
-                const int slot = 2 * cta + (u == line.begin ? 0 : 1);
-                float *part = a.part + (size_t)(slot * kT + t) * (D + 2) * kRowsTile + row;
+                float *const part = cur.part;
                 if (first < end)
 #pragma unroll
                     for (int xx = 0; xx < D / kGroups; xx += 32) {
@@ -521,12 +564,8 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
             } else if (!alive) {
                 break;
             }
-            if (tid == 0 && first == 0 && last < line.units)      // the tile starts here and goes on: its parts
-                joins[cta] = JoinTile{req.t0, req.n, line.g, line.m, cta, line.cta_of(line.behind() - 1),
-                                      2 * cta + (u == line.begin ? 0 : 1), 1};
-            u = line.behind();
-            if (u >= line.end) break;
-            line.next();
+            cur = next;
+            c = c_next;
         }
     } else if (warp < kMmaWarp) {
         // ================================ load ===================================================
