@@ -2,13 +2,15 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c q.k_j - m)
 //
-// A tile is 128 packed query rows (new token x query head) of one key/value head; a CTA carries two
-// of them (one for dim 256), each with its own scores S and sums O in tensor memory, so that the
-// tensor core multiplies for one while the other's probabilities are computed. Roles:
-//   softmax  one warpgroup per tile, a thread per row: its queries into shared memory, then per block
-//            of keys S -> running maximum -> P, written over S as the next product's A operand. Where a
-//            CTA has one tile, two warpgroups take turns at its blocks; the maximum passes from one to the
-//            other through shared memory, the sums are added at the end
+// A tile is 128 packed query rows (new token x query head) of one key/value head. A CTA carries two of
+// them for bf16 outputs at dims 64 and 128, so that the tensor core multiplies for one while the other's
+// probabilities are computed, else one: dim 256 and the lower terms of fp32 outputs need the tensor
+// memory. Each tile has its own scores S and sums O there. Roles:
+//   softmax  one warpgroup per tile, a thread per row: its queries into shared memory (the next tile's
+//            under the end of the last), then per block of 64 keys S -> running maximum -> P, written over
+//            S as the next product's A operand. Where a CTA has one tile, two warpgroups take turns at its
+//            blocks; the maximum passes from one to the other through shared memory, the sums are added
+//            at the end
 //   load     the blocks of keys and values, page by page, into a ring in shared memory: one warp that
 //            issues TMA copies of 8 to 64 rows, or, where pages are no multiple of 8 or the cache is
 //            e4m3 (which becomes fp16 on the way), four warps through their registers
@@ -18,8 +20,13 @@
 // O is rescaled only when a row's maximum grows by more than 2^8: until then probabilities are up to
 // 2^8 instead of 1, which costs no precision, and the rescaling pass over O hardly ever runs.
 //
-// Two products of 128 x 128 x dim and 128 x 128 exponentials take about the same time on an SM
-// (1024 clocks at dim 128), which bounds this kernel; the cache is read once per 256 rows.
+// What bounds it. bf16 outputs: the products of two tiles and 64 keys take 1024 clocks at dim 128, their
+// 16384 exponentials as long on the special-function units, next to maxima, sums and packing on the same
+// four warps a tile: the softmax warpgroups set the pace. One pair of exponentials in four goes to the FMA
+// pipe. 4096 new tokens (32 query, 8 key/value heads of 128): 462 us = 0.67 of the measured bf16 rate by
+// operations (311 us). fp32 outputs carry P in three terms, four products instead of two: a batch of
+// chunks and decodes takes 273 us, 0.40 of the rate by the operations issued (110 us); there the split of P
+// into terms, 12 instructions a pair, takes longer than the products. One warpgroup a tile: 303 us.
 //
 // Work is cut into equal stretches of key blocks, one per SM (Line, kv.cuh): a causal batch of any
 // lengths loads all SMs alike. A tile cut between CTAs leaves (m, sum, O) of each part in global
@@ -40,7 +47,7 @@ namespace {
 constexpr int kRowsTile = 128;
 // How the load warps bring a block in.
 enum Load { kTma, kRegs, kRegsE4m3 };
-constexpr int kCubic = 2;             // of four pairs of exponentials, those that the FMA pipe computes
+constexpr int kCubic = 1;             // of four pairs of exponentials, those that the FMA pipe computes (0, 1, 2, 3: 480, 462, 481, 522 us at 4096 tokens)
 
 template <int D, Load LOAD, int TERMS>
 struct TileShape {
