@@ -172,7 +172,8 @@ void tq_sync(void) {
         if (cudaMemcpy(&st, tq::g_status_dev, sizeof(int), cudaMemcpyDeviceToHost) == cudaSuccess &&
             st != 0) {
             tq::g_sticky_error = 10000 + st;
-            fprintf(stderr, "forward_qwen_xpu(b200): device wait gave up, status %d\n", st);
+            fprintf(stderr, "forward_qwen_xpu(b200): %s, status %d\n",
+                    st >= 41 && st <= 43 ? "impossible numbers in a call's device arrays" : "device wait gave up", st);
         }
     }
 }

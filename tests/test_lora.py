@@ -180,6 +180,47 @@ def test_lora_in_a_graph(lib, pkg):
     _check([ref.down(y, torch.float32, f.shape) for y, f in zip(ys, first)], c)
 
 
+GROWTH = """
+import ctypes as C, importlib, sys
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+import torch
+import attnref as ref
+from test_lora import _make, _run, _check
+pkg = importlib.import_module("knivesysl-xe_b200")
+lib = pkg.load()
+assert lib.tq_set_device(0) == 0
+c = _make(pkg, 1, 2, 8, [64], 64, 3, [0, 1, 0], seed=1)
+_run(lib, pkg, c)
+x, ids, base, y = ref.up(c["x"]), ref.up(c["ids"]), ref.up(c["w"][0]["base"]), ref.up(c["w"][0]["base"])
+assert lib.tq_graph_capture_begin() == 0
+assert lib.qwn_x_lora_add(pkg.lora_array([c["w"][0]["rec"]]), ref.ptrs([base]), ref.ptrs([y]), 1, x.ptr, ids.ptr, 3) == 0
+graph = lib.tq_graph_capture_end()
+keep = []
+for T in (70, 600, 3000):                  # each wants more scratch than the last
+    d = _make(pkg, 2, 2, 128, [64, 64], 128, T, [t % 2 for t in range(T)], seed=T)
+    _check(_run(lib, pkg, d), d)
+    other = pkg.DevBuf(1 << 16)            # would take the place of what was freed
+    lib.tq_dev_fill(other.ptr, 0x5a, other.nbytes)
+    keep.append(other)
+lib.tq_graph_launch(graph)
+lib.tq_sync()
+lib.tq_graph_destroy(graph)
+_check([ref.down(y, torch.float32, (3, 64))], c)
+for other in keep:
+    assert (other.to_numpy("uint8", 1 << 16) == 0x5a).all()
+assert lib.tq_last_error() == 0
+print("ok")
+"""
+
+
+@pytest.mark.gpu
+def test_a_captured_call_outlives_larger_ones(lib):
+    """The scratch that a graph was captured with is not given back when a larger call makes a new one."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", GROWTH.format(root=root)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.splitlines() == ["ok"], out.stderr
+
+
 FIRST_CALL = """
 import ctypes as C, importlib, sys
 sys.path.insert(0, {root!r})
@@ -192,7 +233,7 @@ lib.tq_sync()
 p = buf.ptr
 cache = pkg.KvCache(p, p + 65536, 4, 16, 2, 64, 0, 1.0, 1.0)
 batch = pkg.KvBatch(1, 1, 1, 4, p, p, p)
-one = (C.c_void_p * 1)(p)
+one = (C.c_void_p * 1)(p + 262144)
 ws = pkg.lora_array([pkg.Lora(1, 8, 16, 32, p, p, None, None)])
 calls = dict(
     append=lambda: lib.qwn_x_kv_append(C.byref(cache), C.byref(batch), None, None, 0, 0, None, p, 128, p, 128),
@@ -246,3 +287,11 @@ def test_lora_refuses_bad_arguments(pkg):
     pair = (C.c_void_p * 2)(4096, 4096)
     assert lib.qwn_x_lora_add(two, pair, pair, 2, 4096, 4096, 4) == -2
     assert lib.qwn_x_lora_add(ws, one, one, 1, 4096, 4096, 0) == 0
+    # one output twice, an output that is another projection's base, one that is x, more rows of B than 32 bits count
+    same = pkg.lora_array([pkg.Lora(**rec)] * 2)
+    ys = lambda *p: (C.c_void_p * 2)(*p)
+    assert lib.qwn_x_lora_add(same, None, ys(8192, 8192), 2, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(same, ys(12288, 8192), ys(8192, 12288), 2, 4096, 4096, 4) == -2
+    assert lib.qwn_x_lora_add(ws, None, one, 1, 4096, 4096, 4) == -2
+    wide = pkg.lora_array([pkg.Lora(**(rec | dict(count=2048, M=1 << 20)))])
+    assert lib.qwn_x_lora_add(wide, None, (C.c_void_p * 1)(8192), 1, 4096, 4096, 4) == -3
