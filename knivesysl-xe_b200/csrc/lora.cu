@@ -30,6 +30,7 @@ constexpr int kTokE = 32;             // and of the expand kernel
 constexpr int kMaxTokens = 4096;      // of a launch
 constexpr size_t kSmemMost = 232448 - 1024;   // dynamic shared memory of a CTA, beside some static
 constexpr int kMaxRank = 256;
+constexpr int kMaxSplits = 8;         // parts of K (with 10: 1000 tokens of 5 adapters 0.3 us less, 64 of 24 and 4096 of 8 1 and 1.6 us more)
 
 struct LoraArgs {
     const uint16_t *a[4], *b[4];
@@ -43,7 +44,7 @@ struct LoraArgs {
     const float *x;
     const int *adapter;
     float *h;                         // [splits][T][hoff[count]]
-    int splits;                       // parts of K, summed in ascending order by the expand kernel
+    int max_splits, sms;              // parts of K at most, SMs: see Plan::splits
     int *status;
 };
 
@@ -65,17 +66,22 @@ __device__ __forceinline__ int rank_of(const LoraArgs &a, int i, int id) {
 // so that every CTA sees the same tiles.
 template <int TOK>
 struct Plan {
-    int *s_off, *s_cnt, *s_list, *s_sum;
+    int *s_off, *s_cnt, *s_list, *s_sum, *s_tiles;
     uint16_t *s_id;
     __device__ Plan(const LoraArgs &a, uint8_t *smem) {
         s_list = reinterpret_cast<int *>(smem);
         s_sum = s_list + TOK;
-        s_off = s_sum + kW;
+        s_tiles = s_sum + kW;
+        s_off = s_tiles + 1;
         s_cnt = s_off + a.adapters + 2;
         s_id = reinterpret_cast<uint16_t *>(s_cnt + a.adapters + 1);
     }
-    static size_t bytes(int adapters, int T) { return ((size_t)TOK + kW + 2 * adapters + 3) * 4 + ((size_t)T + 1) / 2 * 4; }
+    static size_t bytes(int adapters, int T) { return ((size_t)TOK + kW + 2 * adapters + 4) * 4 + ((size_t)T + 1) / 2 * 4; }
     __device__ int tokens(int g, int tile) const { return min(TOK, s_cnt[g] - (tile - s_off[g]) * TOK); }
+
+    // Parts that K is cut into, the same in both kernels: as many as make one round of CTAs of the shrink kernel's
+    // tasks. A task's fixed cost (its tokens, its rank, filling the rings, adding the warps' sums) is several us.
+    __device__ int splits(const LoraArgs &a) const { return max(1, min(a.max_splits, a.sms / max(1, *s_tiles * a.count))); }
 
     // All threads of the CTA, of which the first kW warps work. Loops are kept short: code that runs once per launch
     // is fetched from far away, and unrolled it costs more than it saves.
@@ -109,10 +115,11 @@ struct Plan {
         }
         __syncthreads();
         if (threadIdx.x < 32) {                      // exclusive scan of the groups' tiles
-            int tiles = 0;
+            int tiles = 0, tiles_shrink = 0;
 #pragma unroll 1
             for (int g0 = 0; g0 <= groups; g0 += 32) {
                 const int g = g0 + lane, m = g < groups ? (s_cnt[g] + TOK - 1) / TOK : 0;
+                if (g >= 1 && g < groups) tiles_shrink += (s_cnt[g] + kTok - 1) / kTok;
                 int sum = m;
 #pragma unroll 1
                 for (int off = 1; off < 32; off <<= 1) {
@@ -122,6 +129,8 @@ struct Plan {
                 if (g <= groups) s_off[g] = tiles + sum - m;
                 tiles += __shfl_sync(0xffffffffu, sum, 31);
             }
+            tiles_shrink = __reduce_add_sync(0xffffffffu, tiles_shrink);
+            if (lane == 0) *s_tiles = tiles_shrink;
         }
         __syncthreads();
     }
@@ -190,13 +199,13 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
     plan.make(a);
     const int tile0 = plan.s_off[1], tiles = plan.s_off[a.adapters + 1] - tile0;      // group 0 has no product
     const int width = a.hoff[a.count], K64 = (a.K + 63) / 64;
-    const int per = a.count * a.splits;
+    const int splits = plan.splits(a), per = a.count * splits;
     for (int task = blockIdx.x; task < tiles * per; task += gridDim.x) {
-        const int tile = tile0 + task / per, i = task % per / a.splits, part = task % a.splits;
+        const int tile = tile0 + task / per, i = task % per / splits, part = task % splits;
         const int g = group_of(a, plan, tile), id = g - 1, tokens = plan.tokens(g, tile);
         if (task == (int)blockIdx.x || tile != tile0 + (task - (int)gridDim.x) / per) plan.list(a, g, tile);
         const int rank = rank_of(a, i, id), R = a.R[i];
-        const int k0 = (int)((long long)K64 * part / a.splits), k1 = (int)((long long)K64 * (part + 1) / a.splits);
+        const int k0 = (int)((long long)K64 * part / splits), k1 = (int)((long long)K64 * (part + 1) / splits);
         const int groups16 = (tokens + 15) / 16, slices = groups16 == 1 ? 8 : (groups16 == 2 ? 4 : 2);
         const int team = kW / slices, slice = warp / team, m = warp % team;    // m >= groups16: nothing to multiply (three groups)
         const int steps = (k1 - k0 - slice + slices - 1) / slices;
@@ -390,12 +399,18 @@ __global__ void __launch_bounds__(kThreadsE, 1)
     plan.make(a);
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const int tiles = plan.s_off[a.adapters + 1], width = a.hoff[a.count];
+    const int width = a.hoff[a.count], splits = plan.splits(a);
     int blocks = 0;
-    for (int i = 0; i < a.count; ++i) blocks += (a.M[i] + kCols - 1) / kCols;
+    bool in_place = true;
+    for (int i = 0; i < a.count; ++i) {
+        blocks += (a.M[i] + kCols - 1) / kCols;
+        in_place = in_place && a.base[i] == a.y[i];
+    }
+    // the tiles without an adapter come first; in place there is nothing to do for them
+    const int tile0 = in_place ? plan.s_off[1] : 0, tiles = plan.s_off[a.adapters + 1] - tile0;
     const int total = tiles * blocks;                // below 2^31 (checked by the entry point)
     const int begin = (int)((long long)total * blockIdx.x / gridDim.x), end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
-    int tile = begin / blocks, c = begin % blocks, i = 0, have_tile = -1, g = 0;
+    int tile = tile0 + begin / blocks, c = begin % blocks, i = 0, have_tile = -1, g = 0;
     while (c >= (a.M[i] + kCols - 1) / kCols) c -= (a.M[i++] + kCols - 1) / kCols;
     int at = 0, task_no = 0, fixes = 0;              // stages of B so far, tasks with a product, mended stages
     auto hold = [&](uint32_t bar, uint32_t parity) { // by any threads of a warp
@@ -448,12 +463,12 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                 float v[2] = {0.0f, 0.0f};
                 if (tok < tokens && r < rank) {
                     const float *h = a.h + (size_t)plan.s_list[tok] * width + a.hoff[i] + r;
-                    float2 part[8];                  // at most 8 parts, all loads under way together
+                    float2 part[kMaxSplits];         // all loads under way together
 #pragma unroll
-                    for (int s = 0; s < 8; ++s)
-                        part[s] = s < a.splits ? __ldcg(reinterpret_cast<const float2 *>(h + (size_t)s * a.T * width)) : make_float2(0.0f, 0.0f);
+                    for (int s = 0; s < kMaxSplits; ++s)
+                        part[s] = s < splits ? __ldcg(reinterpret_cast<const float2 *>(h + (size_t)s * a.T * width)) : make_float2(0.0f, 0.0f);
 #pragma unroll
-                    for (int s = 0; s < 8; ++s) {
+                    for (int s = 0; s < kMaxSplits; ++s) {
                         v[0] += part[s].x;
                         v[1] += part[s].y;
                     }
@@ -662,10 +677,10 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
     // a call of more tokens than a CTA sorts goes in pieces
     const int piece = std::min(T, kMaxTokens), k64 = (a.K + 63) / 64;
     const int tiles = (piece + kTok - 1) / kTok + std::min(piece, a.adapters);     // at most
-    // one round of CTAs: a task's fixed cost (its tokens, its rank, filling the rings, adding the warps' sums) is
-    // several us; and a step for every warp at least
-    a.splits = std::max(1, std::min({8, sms / std::max(1, tiles * count), k64 / kW}));
-    const size_t need = (size_t)a.splits * piece * a.hoff[count];
+    // A step for every warp at least. The kernels cut K by the tiles that there are (Plan::splits); this is the most.
+    a.max_splits = std::max(1, std::min({kMaxSplits, sms / ((piece + kTok - 1) / kTok * count), k64 / kW}));
+    a.sms = sms;
+    const size_t need = (size_t)a.max_splits * piece * a.hoff[count];
     if (need > g_h_floats) {
         if (stream_is_capturing()) return -40;
         // The last scratch stays allocated: a graph may have been captured with it. Each is twice the last at least.
@@ -702,7 +717,7 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
             a.base[i] = bases && bases[i] ? bases[i] + (size_t)t0 * a.M[i] : nullptr;
             a.y[i] = ys[i] + (size_t)t0 * a.M[i];
         }
-        const int shrink = (int)std::min<long long>((long long)tiles * count * a.splits, sms);
+        const int shrink = (int)std::min<long long>((long long)tiles * count * a.max_splits, sms);
         const int expand = (int)std::min<long long>(tiles_e * blocks, sms);
         launch_pdl(lora_shrink_kernel, dim3(shrink), dim3(kW * 32), shrink_smem, a);
         launch_pdl(lora_expand_kernel, dim3(expand), dim3(kThreadsE), expand_smem, a, chunks, wait_limit_ns(), maps);
