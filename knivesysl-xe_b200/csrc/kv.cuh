@@ -255,12 +255,11 @@ __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v 
 // Three bf16 terms of each of a pair of fp32 values, cut off instead of rounded: 8 bits each, their sum
 // is the value (of a value that is not finite, NaN).
 __device__ __forceinline__ void split3(float x, float y, uint32_t &t0, uint32_t &t1, uint32_t &t2) {
+    const f32x2 minus = pack2(-1.0f, -1.0f);       // x - term as an exact fma, two at a time
     t0 = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-    x -= bf16_lo(t0);
-    y -= bf16_hi(t0);
+    unpack2(fma2(pack2(__uint_as_float(__float_as_uint(x) & 0xffff0000u), bf16_hi(__float_as_uint(y))), minus, pack2(x, y)), x, y);
     t1 = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-    x -= bf16_lo(t1);
-    y -= bf16_hi(t1);
+    unpack2(fma2(pack2(__uint_as_float(__float_as_uint(x) & 0xffff0000u), bf16_hi(__float_as_uint(y))), minus, pack2(x, y)), x, y);
     t2 = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
 }
 // Two e4m3 values (low byte first) as fp16, exactly.
