@@ -171,14 +171,16 @@ __device__ __forceinline__ int group_of(const LoraArgs &a, const Plan<TOK> &p, i
 }
 
 // ---- shrink ------------------------------------------------------------------------------------
-// A task is (tile, projection, part of K). Its eight warps are shared out over the tile's 1 to 4 groups
+// A task is (tile, projection, part of K). Its warps are shared out over the tile's 1 to 4 groups
 // of 16 tokens and, for each, slices of the part, whose sums are added through shared memory. The warps
 // of a slice bring 64 values of K at a time, each of its 16 rows of x and all together of 64 ranks of A,
 // through a ring of theirs (cp.async, 2 to 4 stages; one barrier of theirs a step). Slices take turns at
 // the 64 values, so that the CTA reads its rows in runs of 512 bytes or more.
-constexpr int kNB = 8;                // groups of 8 ranks per pass
-constexpr int kXBytes = 16 * 256, kABytes = kNB * 8 * 128;
-constexpr int kRingBytes = kW * 2 * (kXBytes + kABytes);          // of the CTA
+// NB groups of 8 ranks per pass, W warps. The products of 64 ranks keep the tensor cores of mma.sync busy with eight
+// warps and their sums fill the registers; up to 32 ranks sixteen warps fit, and they hide more of the latency of
+// splitting x.
+constexpr int kXBytes = 16 * 256;
+constexpr int kRingBytes = 196608;    // of the CTA
 
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     uint4 v;
@@ -189,9 +191,12 @@ __device__ __forceinline__ void cp_async16_live(uint32_t dst, const void *src, b
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-__global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs a) {
+template <int NB, int W>
+__global__ void __launch_bounds__(W * 32, 1) lora_shrink_kernel(const LoraArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
-    auto sums = [&](int w) { return reinterpret_cast<float (*)[kNB * 8 + 2]>(smem + w * (kRingBytes / kW)); };   // over the rings
+    constexpr int kABytes = NB * 8 * 128;
+    static_assert(kRingBytes / 8 >= 2 * (W / 8 * kXBytes + kABytes) && kRingBytes / W >= 16 * (NB * 8 + 2) * 4, "");
+    auto sums = [&](int w) { return reinterpret_cast<float (*)[NB * 8 + 2]>(smem + w * (kRingBytes / W)); };   // over the rings
     const Plan<kTok> plan(a, smem + kRingBytes);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, row = lane >> 2;
     pdl_wait();
@@ -206,8 +211,8 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
         if (task == (int)blockIdx.x || tile != tile0 + (task - (int)gridDim.x) / per) plan.list(a, g, tile);
         const int rank = rank_of(a, i, id), R = a.R[i];
         const int k0 = (int)((long long)K64 * part / splits), k1 = (int)((long long)K64 * (part + 1) / splits);
-        const int groups16 = (tokens + 15) / 16, slices = groups16 == 1 ? 8 : (groups16 == 2 ? 4 : 2);
-        const int team = kW / slices, slice = warp / team, m = warp % team;    // m >= groups16: nothing to multiply (three groups)
+        const int groups16 = (tokens + 15) / 16, slices = min(8, groups16 == 1 ? W : (groups16 == 2 ? W / 2 : W / 4));
+        const int team = W / slices, slice = warp / team, m = warp % team;    // m >= groups16: nothing to multiply (three groups)
         const int steps = (k1 - k0 - slice + slices - 1) / slices;
         const int stage_bytes = team * kXBytes + kABytes, stages = kRingBytes / slices / stage_bytes;      // 2, 3 or 4
         const uint32_t ring = smem_u32(smem) + slice * (kRingBytes / slices);
@@ -218,8 +223,8 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
             const int tok = m * 16 + c * 2 + (lane >> 4);
             xt[c] = tok < tokens ? plan.s_list[tok] : -1;
         }
-        for (int r0 = 0; r0 < rank; r0 += kNB * 8) {
-            const int nb = min(kNB, (rank - r0 + 7) / 8);
+        for (int r0 = 0; r0 < rank; r0 += NB * 8) {
+            const int nb = min(NB, (rank - r0 + 7) / 8);
             const uint16_t *A = a.a[i] + ((size_t)id * R + r0) * a.K;
             auto issue = [&](int s) {
                 if (s < steps) {
@@ -242,9 +247,9 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
                 cp_async_commit();
             };
             for (int s = 0; s < stages - 1; ++s) issue(s);
-            float acc[kNB][4], sum[kNB][4];
+            float acc[NB][4], sum[NB][4];
 #pragma unroll
-            for (int n = 0; n < kNB; ++n)
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[n][e] = sum[n][e] = 0.0f;
             for (int s = 0; s < steps; ++s) {
@@ -269,9 +274,9 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
                             split3(__uint_as_float(v.z), __uint_as_float(v.w), f[z][0][2 + h], f[z][1][2 + h], f[z][2][2 + h]);
                         }
                     }
-                    uint4 w[kNB];
+                    uint4 w[NB];
 #pragma unroll
-                    for (int n = 0; n < kNB; ++n) {
+                    for (int n = 0; n < NB; ++n) {
                         const int r = n * 8 + row;
                         if (n < nb) w[n] = lds16(src + r * 128 + (((half * 4 + quad) ^ (r & 1) << 2) << 4));
                     }
@@ -279,16 +284,16 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
 #pragma unroll
                     for (int z = 0; z < 3; ++z) {
 #pragma unroll
-                        for (int n = 0; n < kNB; ++n)
+                        for (int n = 0; n < NB; ++n)
                             if (n < nb) mma_bf16(acc[n], f[0][z], w[n].x, w[n].y);
 #pragma unroll
-                        for (int n = 0; n < kNB; ++n)
+                        for (int n = 0; n < NB; ++n)
                             if (n < nb) mma_bf16(acc[n], f[1][z], w[n].z, w[n].w);
                     }
                 }
                 if ((s & 1) || s + 1 == steps) {
 #pragma unroll
-                    for (int n = 0; n < kNB; ++n)
+                    for (int n = 0; n < NB; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             sum[n][e] += acc[n][e];
@@ -299,13 +304,13 @@ __global__ void __launch_bounds__(kW * 32, 1) lora_shrink_kernel(const LoraArgs 
             cp_async_wait<0>();
             __syncthreads();                              // the rings are free
 #pragma unroll
-            for (int n = 0; n < kNB; ++n)
+            for (int n = 0; n < NB; ++n)
                 if (n < nb) {
                     *reinterpret_cast<float2 *>(&sums(warp)[row][n * 8 + quad * 2]) = make_float2(sum[n][0], sum[n][1]);
                     *reinterpret_cast<float2 *>(&sums(warp)[row + 8][n * 8 + quad * 2]) = make_float2(sum[n][2], sum[n][3]);
                 }
             __syncthreads();
-            for (int e = threadIdx.x; e < tokens * nb * 8; e += kW * 32) {
+            for (int e = threadIdx.x; e < tokens * nb * 8; e += W * 32) {
                 const int i_tok = e / (nb * 8), r = e % (nb * 8), t = plan.s_list[i_tok];
                 float s = 0.0f;
                 for (int w = 0; w < slices; ++w) s += sums(w * team + (i_tok >> 4))[i_tok & 15][r];
@@ -705,7 +710,8 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
     const size_t expand_smem = 1024 + (size_t)kRing * kBlockB + (size_t)chunks * kHTile + Plan<kTokE>::bytes(a.adapters, piece);
     static bool set = false;
     if (!set) {
-        TQ_CHECK(cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
+        TQ_CHECK(cudaFuncSetAttribute(lora_shrink_kernel<4, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
+        TQ_CHECK(cudaFuncSetAttribute(lora_shrink_kernel<8, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
         TQ_CHECK(cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
         set = true;
     }
@@ -719,7 +725,8 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
         }
         const int shrink = (int)std::min<long long>((long long)tiles * count * a.max_splits, sms);
         const int expand = (int)std::min<long long>(tiles_e * blocks, sms);
-        launch_pdl(lora_shrink_kernel, dim3(shrink), dim3(kW * 32), shrink_smem, a);
+        if (most <= 32) launch_pdl(lora_shrink_kernel<4, 16>, dim3(shrink), dim3(16 * 32), shrink_smem, a);
+        else launch_pdl(lora_shrink_kernel<8, 8>, dim3(shrink), dim3(8 * 32), shrink_smem, a);
         launch_pdl(lora_expand_kernel, dim3(expand), dim3(kThreadsE), expand_smem, a, chunks, wait_limit_ns(), maps);
     }
     TQ_LAUNCH_CHECK("lora_expand_kernel");
