@@ -30,7 +30,7 @@ constexpr int kTokE = 32;             // and of the expand kernel
 constexpr int kMaxTokens = 4096;      // of a launch
 constexpr size_t kSmemMost = 232448 - 1024;   // dynamic shared memory of a CTA, beside some static
 constexpr int kMaxRank = 256;
-constexpr int kMaxSplits = 8;         // parts of K (with 10: 1000 tokens of 5 adapters 0.3 us less, 64 of 24 and 4096 of 8 1 and 1.6 us more)
+constexpr int kMaxSplits = 16;        // parts of K
 
 struct LoraArgs {
     const uint16_t *a[4], *b[4];
@@ -178,7 +178,8 @@ __device__ __forceinline__ int group_of(const LoraArgs &a, const Plan<TOK> &p, i
 // the 64 values, so that the CTA reads its rows in runs of 512 bytes or more.
 // NB groups of 8 ranks per pass, W warps. The products of 64 ranks keep the tensor cores of mma.sync busy with eight
 // warps and their sums fill the registers; up to 32 ranks sixteen warps fit, and they hide more of the latency of
-// splitting x.
+// splitting x: 16, 64, 128 and 1000 tokens of 5 adapters of rank 32, K 17408, take 22.0, 23.6, 32.2 and 50 us with
+// sixteen, 20.3, 22.0, 41.0 and 59 us with eight, which therefore serve decode batches (up to 64 tokens).
 constexpr int kXBytes = 16 * 256;
 constexpr int kRingBytes = 196608;    // of the CTA
 
@@ -468,14 +469,17 @@ __global__ void __launch_bounds__(kThreadsE, 1)
                 float v[2] = {0.0f, 0.0f};
                 if (tok < tokens && r < rank) {
                     const float *h = a.h + (size_t)plan.s_list[tok] * width + a.hoff[i] + r;
-                    float2 part[kMaxSplits];         // all loads under way together
+#pragma unroll 1
+                    for (int s0 = 0; s0 < splits; s0 += 8) {
+                        float2 part[8];              // all loads under way together
 #pragma unroll
-                    for (int s = 0; s < kMaxSplits; ++s)
-                        part[s] = s < splits ? __ldcg(reinterpret_cast<const float2 *>(h + (size_t)s * a.T * width)) : make_float2(0.0f, 0.0f);
+                        for (int s = 0; s < 8; ++s)
+                            part[s] = s0 + s < splits ? __ldcg(reinterpret_cast<const float2 *>(h + (size_t)(s0 + s) * a.T * width)) : make_float2(0.0f, 0.0f);
 #pragma unroll
-                    for (int s = 0; s < kMaxSplits; ++s) {
-                        v[0] += part[s].x;
-                        v[1] += part[s].y;
+                        for (int s = 0; s < 8; ++s) {
+                            v[0] += part[s].x;
+                            v[1] += part[s].y;
+                        }
                     }
                 }
                 v[0] = r < rank ? v[0] * scale : 0.0f;
@@ -725,7 +729,7 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
         }
         const int shrink = (int)std::min<long long>((long long)tiles * count * a.max_splits, sms);
         const int expand = (int)std::min<long long>(tiles_e * blocks, sms);
-        if (most <= 32) launch_pdl(lora_shrink_kernel<4, 16>, dim3(shrink), dim3(16 * 32), shrink_smem, a);
+        if (most <= 32 && piece > kTok) launch_pdl(lora_shrink_kernel<4, 16>, dim3(shrink), dim3(16 * 32), shrink_smem, a);
         else launch_pdl(lora_shrink_kernel<8, 8>, dim3(shrink), dim3(8 * 32), shrink_smem, a);
         launch_pdl(lora_expand_kernel, dim3(expand), dim3(kThreadsE), expand_smem, a, chunks, wait_limit_ns(), maps);
     }
