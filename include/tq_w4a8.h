@@ -457,7 +457,8 @@ int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, con
                      float scale, void *d_out, size_t ldo, int out_bf16);
 /* ys[i][t] = bases[i][t] + scale (x[t] A^T) B^T with the adapter d_adapter[t] of ws[i] (negative: none, the row is
  * bases[i][t]); up to 4 projections of one input, with the same K and number of adapters. x fp32 [T][K], bases and
- * ys fp32 [T][M]; bases[i] may be ys[i] (added in place) or NULL, as may bases (0). Products and sums are fp32's.
+ * ys fp32 [T][M]; bases[i] may be ys[i] (added in place) or NULL, as may bases (0). Products and sums are fp32's; an
+ * infinity in x makes its row NaN.
  * No output may be x, another output or another projection's base (-2). M is at most 2^21 and count * M below 2^31
  * (-3). An adapter number beyond the pool or a rank out of range counts as none and leaves 10043 in tq_last_error().
  * The scratch grows with T (up to 4096) and the ranks; what a captured graph uses stays. Returns as x_kv_append. */

@@ -14,9 +14,9 @@
 // by the last of them to finish, in the order of the keys, so results do not depend on timing.
 //
 // The rule: at most 16 packed rows a head. Decoding through the kernel of 128-row tiles instead takes 38 us
-// for one request, 159 us for 64 (here 13.5 and 68) and 187 us for 8 long e4m3 caches (here 73): its ring
+// for one request, 159 us for 64 (here 13.5 and 65) and 187 us for 8 long e4m3 caches (here 73): its ring
 // and its barriers wait for 128 rows of products where 16 are wanted. Above 16 rows this one would read the
-// cache again for every 16. Measured: 64 requests, bf16, 336 MB of cache: 68 us, 4.9 TB/s; 8 long e4m3
+// cache again for every 16. Measured: 64 requests, bf16, 336 MB of cache: 65 us, 5.2 TB/s; 8 long e4m3
 // caches of dim 256, 171 MB: 73 us, 2.3 TB/s, where turning e4m3 into fp16 (a conversion per two values at
 // a quarter rate) and the latency of two blocks in flight a warp weigh more than the bytes; one request:
 // 13.5 us, latency of launch, first bytes and join.

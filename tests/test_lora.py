@@ -82,6 +82,8 @@ CASES = [
     ([64, 32, 16, 48], 300, 8, 64, 200),
     ([2560, 1296], 3, 72, 64, 3000),
     ([1920], 30, 64, 96, 4500),
+    ([96], 3, 24, 9248, 40),
+    ([64, 48], 2, 32, 1120, 333),
 ]
 
 
