@@ -112,6 +112,17 @@ def test_lora_orders_of_tokens(lib, pkg, ids):
 
 
 @pytest.mark.gpu
+def test_lora_in_place_without_any_adapter(lib, pkg):
+    """Nothing to do for any row: all of them keep their bits, and the next call works."""
+    c = _make(pkg, 2, 4, 16, [96, 80], 160, 70, [-1] * 70, seed=4)
+    for y, w in zip(_run(lib, pkg, c, "inplace"), c["w"]):
+        assert torch.equal(y, w["base"])
+    c = _make(pkg, 2, 4, 16, [96, 80], 160, 70, [t % 5 - 1 for t in range(70)], seed=5)
+    _check(_run(lib, pkg, c, "inplace"), c)
+    assert lib.tq_last_error() == 0
+
+
+@pytest.mark.gpu
 def test_lora_rows_do_not_depend_on_their_company(lib, pkg):
     """Values that are not finite stay in their own token's row, and a token's bits do not depend on who
     shares its tile."""
