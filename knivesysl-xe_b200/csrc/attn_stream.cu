@@ -25,7 +25,8 @@
 // cache: e4m3 is exact in fp16, and a query row times a power of two that brings its largest value
 // to [2^9, 2^10) loses only what lies 2^-34 below that). Probabilities enter the second product as
 // one bf16 term for bf16 outputs (fp16 with an e4m3 cache), and for fp32 outputs as three bf16 terms
-// or two fp16 ones, 24 and 22 bits. All sums are fp32.
+// or two fp16 ones, 24 and 22 bits. All sums are fp32; for fp32 outputs they leave the tensor core, which
+// cuts them off, after every block of 16 keys.
 #include "attn.cuh"
 
 #include <algorithm>
@@ -74,6 +75,19 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same on top of nothing.
+template <bool F16>
+__device__ __forceinline__ void mma16816_fresh(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 template <int D, bool E4M3, bool OUT_BF16>
@@ -297,26 +311,46 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
             const int vkey = (lane & 7) + ((lane >> 3) & 1) * 8;
             const int vswz = (((vkey & 1) << 2) | ((vkey >> 1) & 3)) & (kChunks - 1);
             const uint32_t vline = kb + (kKeys + vkey) * S::kRowBytes;
+            // A step takes 2 or 4 chunks, four n8 tiles of o. An e4m3 unit holds two neighbouring dims of a key; bytes 0, 2
+            // and 1, 3 pair the keys
+            constexpr int kPer = E4M3 ? 2 : 1, kStep = 4 / kPer, kOut = 4;       // n8 tiles of a chunk, chunks and tiles of a step
 #pragma unroll
-            for (int j = 0; j < kChunks; j += 2) {
-                uint32_t w[4];
-                ldmatrix_x4_trans(vline + (((j + (lane >> 4)) ^ vswz) << 4), w);
+            for (int j = 0; j < kChunks; j += kStep) {
+                uint32_t w[kStep / 2][4];              // chunk j + i: words 2i (keys 0-7) and 2i + 1 (keys 8-15)
 #pragma unroll
-                for (int k = 0; k < kTerms; ++k)
+                for (int i = 0; i < kStep / 2; ++i) ldmatrix_x4_trans(vline + (((j + 2 * i + (lane >> 4)) ^ vswz) << 4), w[i]);
+                uint32_t v[kOut][2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {      // chunk j + i: w[2i] keys 0-7, w[2i + 1] keys 8-15
-                        if constexpr (E4M3) {
-                            // a unit holds two neighbouring dims of a key; bytes 0, 2 and 1, 3 pair the keys
+                for (int n = 0; n < kOut; ++n)
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const uint32_t sel = x ? 0x4431u : 0x4420u;
-                                mma16816<true>(o[(j + i) * 2 + x], pf[k], e4m3_to_f16((uint16_t)__byte_perm(w[2 * i], 0, sel)),
-                                               e4m3_to_f16((uint16_t)__byte_perm(w[2 * i + 1], 0, sel)));
-                            }
-                        } else {
-                            mma16816<false>(o[j + i], pf[k], w[2 * i], w[2 * i + 1]);
-                        }
+                    for (int y = 0; y < 2; ++y) {
+                        const int chunk = n / kPer;
+                        const uint32_t u16 = w[chunk / 2][chunk % 2 * 2 + y];
+                        if constexpr (E4M3) v[n][y] = e4m3_to_f16((uint16_t)__byte_perm(u16, 0, n & 1 ? 0x4431u : 0x4420u));
+                        else v[n][y] = u16;
                     }
+                if constexpr (kTerms == 1) {
+#pragma unroll
+                    for (int n = 0; n < kOut; ++n) mma16816<E4M3>(o[j * kPer + n], pf[0], v[n][0], v[n][1]);
+                } else {
+                    // The tensor core cuts an fp32 sum off instead of rounding it, so a long one falls behind (4e-5 to 9e-5
+                    // of itself after 17000 keys): a block's terms, the lower first, have a sum of their own, which an
+                    // ordinary addition takes to o (5e-7). 64 decodes: 68 -> 70 us
+                    float d[kOut][4];
+#pragma unroll
+                    for (int n = 0; n < kOut; ++n) mma16816_fresh<E4M3>(d[n], pf[kTerms - 1], v[n][0], v[n][1]);
+#pragma unroll
+                    for (int k = kTerms - 2; k >= 0; --k)
+#pragma unroll
+                        for (int n = 0; n < kOut; ++n) mma16816<E4M3>(d[n], pf[k], v[n][0], v[n][1]);
+#pragma unroll
+                    for (int n = 0; n < kOut; ++n)
+#pragma unroll
+                        for (int x = 0; x < 4; x += 2) {
+                            float (&y)[4] = o[j * kPer + n];
+                            unpack2(add2(pack2(y[x], y[x + 1]), pack2(d[n][x], d[n][x + 1])), y[x], y[x + 1]);
+                        }
+                }
             }
         }
         cp_async_wait<0>();

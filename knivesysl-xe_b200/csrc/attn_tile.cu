@@ -32,7 +32,7 @@
 // lengths loads all SMs alike. A tile cut between CTAs leaves (m, sum, O) of each part in global
 // memory, and a second, small kernel joins them in the order of the keys.
 //
-// Roundings: as in attn_stream.cu.
+// Roundings: as in attn_stream.cu. Every 256 to 8192 keys (kSeg) the sums O are added to fp32 sums outside tensor memory.
 #include "attn.cuh"
 #include "tc.cuh"
 
@@ -63,6 +63,13 @@ struct TileShape {
     // block j are done; more terms of P leave room for one only.
     static constexpr int kBuf = kTiles == 1 || TERMS == 1 ? 2 : 1;
     static constexpr int kSlotCols = 256 / (kTiles * kBuf);
+    // Blocks that O sums up in tensor memory before it goes to fp32 sums outside. The tensor core cuts an fp32 sum off, by up
+    // to 2^-23 of it, twice in a step of 16 keys: n cuts of a sum that grows evenly take n 2^-24. fp32 outputs: 128 cuts at
+    // most, and 4e-6 was the most measured; without it 35000 keys in a row lose 1.5e-4 (two terms), 1.8e-4 (lower terms
+    // apart) or 4e-4 (three terms in one sum). bf16 outputs: 140000 keys lost 8e-4 of themselves. Chunks of 1024 and 512
+    // tokens on 3000 and 1500, fp32: 189 -> 203 us at dim 128, 126 -> 134 at 64, 197 -> 258 at 256, where a sum of all
+    // three terms has to leave every 256 keys.
+    static constexpr int kSeg = TERMS == 1 ? 128 : (kLow ? 16 : (TERMS == 2 ? 8 : 4));
     static constexpr int kBlock = kKeys * D * 2;                    // bytes of keys, or of values
     static constexpr int kRing = 131072 / kBlock > 8 ? 8 : 131072 / kBlock;
     static constexpr int kQ = kRowsTile * D * 2;                    // bytes of a tile's queries
@@ -125,6 +132,58 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A row tile's sums in global memory, four dims of a row together: neighbouring threads (rows) take neighbouring 16 bytes.
+// Behind them, as if they were four more, the row's maximum and its sum of weights.
+template <int D>
+constexpr int kPartFloats = (D + 4) * kRowsTile;
+__device__ __forceinline__ float *part_at(float *row, int dim) { return row + dim * kRowsTile; }      // row: the first of its places
+// Written, added to and read by one thread, past L1.
+__device__ __forceinline__ void st_sums(float *p, float4 v) {
+    asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void add_sums(float *p, float4 v) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ float4 ld_sums(const float *p) {
+    float4 v;
+    asm volatile("ld.relaxed.gpu.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
+// COLS dims of a row's sums leave tensor memory for those in global memory (the tile's place among the parts, whether or
+// not it is cut): stored the first time (`once`), then added. Adding without reading has nothing to wait for; one thread's
+// additions to an address keep their order. The sums outside go by the maximum *ref, those in tensor memory by `top`, which
+// is no smaller; grown by more than 2^8, it scales the former first. Out of line: the block loop has no registers to spare.
+template <int COLS>
+static __device__ __noinline__ void flush_sums(float *part, uint32_t o_col, float *ref_at, bool once, float top) {
+    float ref = once ? top : *ref_at;
+    if (__any_sync(0xffffffffu, top > ref + 8.0f)) {
+        const float by = top == -INFINITY ? 1.0f : exp2_approx(ref - top);
+#pragma unroll 2
+        for (int x = 0; x < COLS; x += 4) {
+            float4 v = ld_sums(part_at(part, x));
+            v.x *= by; v.y *= by; v.z *= by; v.w *= by;
+            st_sums(part_at(part, x), v);
+        }
+        ref = top;
+    }
+    *ref_at = ref;
+    const float f = top == -INFINITY ? 0.0f : exp2_approx(top - ref);
+#pragma unroll 1
+    for (int x = 0; x < COLS; x += 32) {
+        uint32_t v[32];
+        tmem_ld32(o_col + x, v);
+        tmem_wait32(v);
+#pragma unroll
+        for (int y = 0; y < 32; y += 4) {
+            const float4 z = make_float4(__uint_as_float(v[y]) * f, __uint_as_float(v[y + 1]) * f, __uint_as_float(v[y + 2]) * f,
+                                         __uint_as_float(v[y + 3]) * f);
+            if (once) st_sums(part_at(part, x + y), z);
+            else add_sums(part_at(part, x + y), z);
+        }
+    }
 }
 
 __device__ __forceinline__ float max3(float x, float y, float z) {
@@ -191,9 +250,10 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ long long s_scan[S::kThreads / 32 + 3];
-    __shared__ __align__(8) uint64_t s_bar[2 * S::kRing + 2 * kScores + 3 * kT + 3];
+    __shared__ __align__(8) uint64_t s_bar[2 * S::kRing + 2 * kScores + 3 * kT + 4];
     __shared__ uint32_t s_tmem;
     __shared__ float s_c[128], s_m[128], s_ml[2][2][128];        // one tile: factor, maximum of each row; (m, l) of each warpgroup
+    __shared__ float s_ref[S::kSoftmax];               // of a thread's row: the maximum that its sums outside tensor memory go by
     __shared__ int s_gave_up, s_stop;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
@@ -211,12 +271,14 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
     const uint32_t drained = bars + 8 * (2 * S::kRing + 2 * kScores + 3 * kT);       // all products and their arrivals are done
 
     const uint32_t m_ready = drained + 16;             // one tile: the maximum up to a block is in s_m
+    const uint32_t flushed = drained + 24;             // one tile: the second warpgroup's share of O has left tensor memory
     const uint32_t landed = drained + 8;               // a block that the load warp has to complete itself
 
     if (tid == 0) {
         mbar_init(drained, kT);
         mbar_init(landed, 1);
         mbar_init(m_ready, 4);
+        mbar_init(flushed, 4);
         for (int i = 0; i < S::kRing; ++i) {
             mbar_init(full(i), S::kLoadWarps);
             mbar_init(empty(i), kT);
@@ -294,7 +356,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
             x.query = x.live ? ((long long)(req.t0 + tok) * a.q_heads + line.g * G + rho % G) * D : -1;
             x.to = (size_t)(req.t0 + tok) * a.ldo + (size_t)(line.g * G + rho % G) * D;
             const int slot = 2 * cta + (u == line.begin ? 0 : 1);
-            x.part = a.part + (size_t)(slot * kT + t) * (D + 2) * kRowsTile + row;
+            x.part = a.part + (size_t)(slot * kT + t) * kPartFloats<D> + row * 4;
             x.behind = line.behind();
             if (tid == 0 && x.first == 0 && x.last > 0 && !x.whole)      // the tile starts here and goes on: its parts
                 joins[cta] = JoinTile{req.t0, req.n, line.g, line.m, cta, line.cta_of(x.behind - 1), slot, 1};
@@ -365,9 +427,13 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
         if (cur.last <= cur.first) cur.end = 0;            // the stretch ends before the tile's first unit
         float c = cur.first < cur.end ? load_q(cur) : 0.0f;
         while (cur.last > cur.first) {
-            const int first = cur.first, end = cur.end, limit = cur.limit, low = cur.low;
+            const int limit = cur.limit, low = cur.low;
             const bool more = cur.behind < line.end, live = cur.live;
             float m = -INFINITY, l = 0.0f, c_next = 0.0f;
+            // This warpgroup's share of O, which has the maximum `top`, leaves for sums outside (see flush_sums).
+            auto flush = [&](bool once, float top) {
+                flush_sums<D / kGroups>(part_at(cur.part, wg * (D / kGroups)), o_col + wg * (D / kGroups), s_ref + tid, once, top);
+            };
             Part next = cur;
             next.last = next.first;                        // none
             auto prepare = [&]() {                         // the stretch's next tile: its queries are on their way under this one's end
@@ -376,117 +442,148 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 next = describe(cur.behind);
                 if (next.last > next.first && next.first < next.end) c_next = load_q(next);
             };
-            if (first < end) {
-                for (int j = first + wg; j < end && alive; j += kGroups) {
-                    const int slot = t * kBuf + (kBuf == 2 ? (j - first) & 1 : 0);
-                    const uint32_t s_col = lane_col + kSlotCol + slot * S::kSlotCols;
-                    if (!wait(s_full(slot), s_phase >> slot & 1)) { alive = false; break; }
-                    s_phase ^= 1u << slot;
-                    tc_fence_after();
-                    const int key0 = j * kN;
-                    const bool cut = key0 + kN - 1 > low;
-                    // ---- maximum of the block
-                    uint32_t v0[32], v1[32];
-                    tmem_ld32(s_col, v0);
-                    tmem_ld32(s_col + 32, v1);
-                    tmem_wait32(v0);
-                    tmem_wait32(v1);
-                    if (cut) {
-#pragma unroll
-                        for (int y = 0; y < 32; ++y) {
-                            if (key0 + y > limit) v0[y] = 0xff800000u;
-                            if (key0 + 32 + y > limit) v1[y] = 0xff800000u;
-                        }
-                    }
-                    float mx = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-                    for (int y = 0; y < 32; y += 2) {
-                        mx = max3(mx, __uint_as_float(v0[y]), __uint_as_float(v0[y + 1]));
-                        mx1 = max3(mx1, __uint_as_float(v1[y]), __uint_as_float(v1[y + 1]));
-                    }
-                    mx = fmaxf(mx, mx1);
-                    mx *= c;
-                    const uint32_t done = blocks_done + (j - first);       // blocks before this one
-                    float before = m;                      // the maximum that O and the blocks before have
-                    if constexpr (kGroups == 2) {
-                        before = -INFINITY;
-                        if (j > first) {
-                            if (!wait(m_ready, (done - 1) & 1)) { alive = false; break; }
-                            before = s_m[row];
-                        }
-                    }
-                    const bool grows = mx > before + 8.0f;
-                    const float now = grows ? mx : before;
-                    if constexpr (kGroups == 2) {
-                        s_m[row] = now;
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(m_ready);
-                    }
-                    if (j > first && __any_sync(0xffffffffu, grows)) {
-                        // The product of block j - 1 must be in O. That of j - 2 is (the scores of block j were
-                        // multiplied behind it), so the barrier is at most one phase behind.
-                        if (!wait(o_done(t), (done - 1) & 1)) { alive = false; break; }
+            if (cur.first < cur.end) {
+                // Every kSeg blocks O leaves for fp32 sums outside. A warpgroup with a tile of its own does that between two
+                // loops over blocks, two that share one from within.
+                for (int seg = cur.first; seg < cur.end && alive;) {
+                    const int seg_end = kGroups == 1 ? min(cur.end, seg + S::kSeg) : cur.end;
+                    for (int j = seg + wg; j < seg_end && alive; j += kGroups) {
+                        const int slot = t * kBuf + (kBuf == 2 ? (j - seg) & 1 : 0);
+                        const uint32_t s_col = lane_col + kSlotCol + slot * S::kSlotCols;
+                        if (!wait(s_full(slot), s_phase >> slot & 1)) { alive = false; break; }
+                        s_phase ^= 1u << slot;
                         tc_fence_after();
-                        const float f = grows ? exp2_approx(before - mx) : 1.0f;
-                        // a short loop: unrolled, its registers push others of the block loop out
-#pragma unroll 1
-                        for (int x = 0; x < (S::kLow ? 2 * D : D); x += 16) {
-                            uint32_t v[16];
-                            tmem_ld16(o_col + x, v);
-                            tmem_wait_ld16(v);
+                        const int key0 = j * kN;
+                        const bool anew = kGroups == 2 && j > seg && (j - seg) % S::kSeg == 0;    // this block's product starts O anew
+                        const bool cut = key0 + kN - 1 > low;
+                        // ---- maximum of the block
+                        uint32_t v0[32], v1[32];
+                        tmem_ld32(s_col, v0);
+                        tmem_ld32(s_col + 32, v1);
+                        tmem_wait32(v0);
+                        tmem_wait32(v1);
+                        if (cut) {
 #pragma unroll
-                            for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) * f);
-                            tmem_st16(o_col + x, v);
+                            for (int y = 0; y < 32; ++y) {
+                                if (key0 + y > limit) v0[y] = 0xff800000u;
+                                if (key0 + 32 + y > limit) v1[y] = 0xff800000u;
+                            }
                         }
-                    }
-                    // this thread's sum so far has the maximum that it last saw
-                    if (now != m) {
-                        l *= exp2_approx(m - now);
-                        m = now;
-                    }
-                    const float off = m == -INFINITY ? 0.0f : -m;
-                    // ---- probabilities, over the scores
-                    f32x2 sum = pack2(0.0f, 0.0f);
-                    const f32x2 c2 = pack2(c, c), off2 = pack2(off, off);
-                    auto weights = [&](const uint32_t (&sc)[32], int x) {
-                        uint32_t w[TERMS][16];
+                        float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
                         for (int y = 0; y < 32; y += 2) {
-                            float p0, p1;
-                            const f32x2 z = fma2(pack2(__uint_as_float(sc[y]), __uint_as_float(sc[y + 1])), c2, off2);
-                            if (TERMS == 1 && (y & 7) >= 8 - 2 * kCubic) {
-                                exp2_cubic(z, p0, p1);
-                            } else {
-                                unpack2(z, p0, p1);
-                                p0 = exp2_approx(p0);
-                                p1 = exp2_approx(p1);
-                            }
-                            sum = add2(sum, pack2(p0, p1));
-                            if constexpr (TERMS == 3) {
-                                split3(p0, p1, w[0][y / 2], w[1][y / 2], w[2][y / 2]);
-                            } else {
-                                w[0][y / 2] = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
-                                if constexpr (TERMS == 2) {
-                                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[0][y / 2]));
-                                    w[1][y / 2] = pack_f16(p0 - f.x, p1 - f.y);
-                                }
+                            mx = max3(mx, __uint_as_float(v0[y]), __uint_as_float(v0[y + 1]));
+                            mx1 = max3(mx1, __uint_as_float(v1[y]), __uint_as_float(v1[y + 1]));
+                        }
+                        mx = fmaxf(mx, mx1);
+                        mx *= c;
+                        const uint32_t done = blocks_done + (j - seg);       // blocks before this one
+                        float before = m;                      // the maximum that O and the blocks before have
+                        if constexpr (kGroups == 2) {
+                            before = -INFINITY;
+                            if (j > seg) {
+                                if (!wait(m_ready, (done - 1) & 1)) { alive = false; break; }
+                                before = s_m[row];
                             }
                         }
-                        tmem_st16(s_col + x / 2, w[0]);
-                        if constexpr (TERMS >= 2) tmem_st16(s_col + 64 + x / 2, w[1]);
-                        if constexpr (TERMS == 3) tmem_st16(s_col + 96 + x / 2, w[2]);
-                    };
-                    weights(v0, 0);
-                    weights(v1, 32);
-                    float l0, l1;
-                    unpack2(sum, l0, l1);
-                    l += l0 + l1;
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full(slot));
+                        const bool grows = mx > before + 8.0f;
+                        const float now = grows ? mx : before;
+                        if constexpr (kGroups == 2) {
+                            s_m[row] = now;
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(m_ready);
+                        }
+                        if (j > seg && (S::kLow || !anew) && __any_sync(0xffffffffu, grows)) {
+                            // The product of block j - 1 must be in O. That of j - 2 is (the scores of block j were
+                            // multiplied behind it), so the barrier is at most one phase behind.
+                            if (!wait(o_done(t), (done - 1) & 1)) { alive = false; break; }
+                            tc_fence_after();
+                            const float f = grows ? exp2_approx(before - mx) : 1.0f;
+                            // a short loop: unrolled, its registers push others of the block loop out
+#pragma unroll 1
+                            for (int x = anew ? D : 0; x < (S::kLow ? 2 * D : D); x += 16) {
+                                uint32_t v[16];
+                                tmem_ld16(o_col + x, v);
+                                tmem_wait_ld16(v);
+#pragma unroll
+                                for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) * f);
+                                tmem_st16(o_col + x, v);
+                            }
+                        }
+                        // this thread's sum so far has the maximum that it last saw
+                        if (now != m) {
+                            l *= exp2_approx(m - now);
+                            m = now;
+                        }
+                        const float off = m == -INFINITY ? 0.0f : -m;
+                        // ---- probabilities, over the scores
+                        f32x2 sum = pack2(0.0f, 0.0f);
+                        const f32x2 c2 = pack2(c, c), off2 = pack2(off, off);
+                        auto weights = [&](const uint32_t (&sc)[32], int x) {
+                            uint32_t w[TERMS][16];
+#pragma unroll
+                            for (int y = 0; y < 32; y += 2) {
+                                float p0, p1;
+                                const f32x2 z = fma2(pack2(__uint_as_float(sc[y]), __uint_as_float(sc[y + 1])), c2, off2);
+                                if (TERMS == 1 && (y & 7) >= 8 - 2 * kCubic) {
+                                    exp2_cubic(z, p0, p1);
+                                } else {
+                                    unpack2(z, p0, p1);
+                                    p0 = exp2_approx(p0);
+                                    p1 = exp2_approx(p1);
+                                }
+                                sum = add2(sum, pack2(p0, p1));
+                                if constexpr (TERMS == 3) {
+                                    split3(p0, p1, w[0][y / 2], w[1][y / 2], w[2][y / 2]);
+                                } else {
+                                    w[0][y / 2] = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+                                    if constexpr (TERMS == 2) {
+                                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[0][y / 2]));
+                                        w[1][y / 2] = pack_f16(p0 - f.x, p1 - f.y);
+                                    }
+                                }
+                            }
+                            tmem_st16(s_col + x / 2, w[0]);
+                            if constexpr (TERMS >= 2) tmem_st16(s_col + 64 + x / 2, w[1]);
+                            if constexpr (TERMS == 3) tmem_st16(s_col + 96 + x / 2, w[2]);
+                        };
+                        weights(v0, 0);
+                        weights(v1, 32);
+                        if (anew) {
+                            // O holds the blocks up to j - 1 (the barrier is at most one phase behind, as above)
+                            if (!wait(o_done(t), (done - 1) & 1)) { alive = false; break; }
+                            tc_fence_after();
+                            flush(j - seg == S::kSeg, before);
+                        }
+                        float l0, l1;
+                        unpack2(sum, l0, l1);
+                        l += l0 + l1;
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_full(slot));
+                        if constexpr (kGroups == 2) {
+                            // The other warpgroup's block starts O anew. Blocks take turns and kSeg is even, so this is always the
+                            // second one. O holds the blocks up to this one; the barrier may be two phases behind.
+                            if (j + 1 < seg_end && (j + 1 - seg) % S::kSeg == 0) {
+                                if (!wait(o_done(t), (done - 1) & 1) || !wait(o_done(t), done & 1)) { alive = false; break; }
+                                tc_fence_after();
+                                flush(j + 1 - seg == S::kSeg, now);
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(flushed);
+                            }
+                        }
+                    }
+                    blocks_done += seg_end - seg;
+                    if (kGroups == 1 && seg_end < cur.end && alive) {
+                        // the product of the last block may be two phases away
+                        if (!wait(o_done(t), blocks_done & 1) || !wait(o_done(t), (blocks_done - 1) & 1)) { alive = false; break; }
+                        tc_fence_after();
+                        flush(seg == cur.first, m);
+                    }
+                    seg = seg_end;
                 }
-                blocks_done += end - first;
                 // With a tile of its own, a warpgroup has seen the scores of the last block: no product reads the
                 // queries any more. Of two, one may not have: there the last product is waited for first.
                 if constexpr (kGroups == 1) prepare();
@@ -505,6 +602,8 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 prepare();
             }
             // ---- the tile's rows, or this CTA's part of them (whatever they hold, if a wait gave up)
+            const bool outside = cur.end - cur.first > S::kSeg;
+            const float f_ref = outside && s_ref[tid] != -INFINITY ? exp2_approx(s_ref[tid] - m) : 0.0f;
             auto load_o = [&](int x, uint32_t (&v)[32]) {
                 tmem_ld32(o_col + x, v);
                 tmem_wait32(v);
@@ -515,11 +614,21 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
 #pragma unroll
                     for (int y = 0; y < 32; ++y) v[y] = __float_as_uint(__uint_as_float(v[y]) + __uint_as_float(w[y]));
                 }
+                if (outside) {
+#pragma unroll
+                    for (int y = 0; y < 32; y += 4) {
+                        const float4 z = ld_sums(part_at(cur.part, x + y));
+                        v[y] = __float_as_uint(fmaf(z.x, f_ref, __uint_as_float(v[y])));
+                        v[y + 1] = __float_as_uint(fmaf(z.y, f_ref, __uint_as_float(v[y + 1])));
+                        v[y + 2] = __float_as_uint(fmaf(z.z, f_ref, __uint_as_float(v[y + 2])));
+                        v[y + 3] = __float_as_uint(fmaf(z.w, f_ref, __uint_as_float(v[y + 3])));
+                    }
+                }
             };
             if (cur.whole) {
                 const float f = l > 0.0f ? __fdiv_rn(a.kv.v_scale, l) : (l == l ? 0.0f : l);
                 const size_t to = cur.to;
-                if (first < end)
+                if (cur.first < cur.end)
 #pragma unroll
                     for (int xx = 0; xx < D / kGroups; xx += 32) {
                         const int x = wg * (D / kGroups) + xx;
@@ -546,20 +655,19 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                         __syncwarp();
                     }
             } else {
-                // [dim][row]: neighbouring threads write neighbouring words
                 float *const part = cur.part;
-                if (first < end)
-#pragma unroll
+                if (cur.first < cur.end)
+#pragma unroll 1
                     for (int xx = 0; xx < D / kGroups; xx += 32) {
                         const int x = wg * (D / kGroups) + xx;
                         uint32_t v[32];
                         load_o(x, v);
 #pragma unroll
-                        for (int y = 0; y < 32; ++y) part[(x + y) * kRowsTile] = __uint_as_float(v[y]);
+                        for (int y = 0; y < 32; y += 4)
+                            *reinterpret_cast<uint4 *>(part_at(part, x + y)) = make_uint4(v[y], v[y + 1], v[y + 2], v[y + 3]);
                     }
                 if (wg == 0) {
-                    part[D * kRowsTile] = m;
-                    part[(D + 1) * kRowsTile] = l;
+                    *reinterpret_cast<float2 *>(part_at(part, D)) = make_float2(m, l);
                 }
             }
             tc_fence_before();
@@ -715,7 +823,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                 *wait.gave_up = 1;
                 return false;
             };
-            uint32_t p_phase = 0, q_phase = 0;             // a bit per score buffer; queries so far
+            uint32_t p_phase = 0, q_phase = 0, flushes = 0;    // a bit per score buffer; queries, flushes so far
             int at = 0;                                    // ring blocks so far (keys and values alternate)
             // descriptors: the word with the address, counted in 16 bytes; a block of the ring, or a tile's
             // queries, is a whole number of those further on
@@ -729,15 +837,18 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                                desc_of(kd + (((k >> 2) * (kN * 128) + (k & 3) * 32) >> 4)), kQkDesc, k > 0);
                 tc_commit(s_full(slot));
             };
-            auto weigh = [&](int slot, int blk, bool fresh, bool closes) {   // O (+)= P V
+            auto weigh = [&](int slot, int blk, bool fresh, bool fresh_low, bool closes) {   // O (+)= P V
                 const uint32_t vd = v_lo + (blk & (S::kRing - 1)) * (S::kBlock >> 4);
                 const uint32_t d = tmem + t * D, p = tmem + kSlotCol + slot * S::kSlotCols;
+                // in one sum the lower terms come first: onto a fresh sum they add without loss
 #pragma unroll
-                for (int z = 0; z < TERMS; ++z)
+                for (int zz = 0; zz < TERMS; ++zz) {
+                    const int z = S::kLow ? zz : TERMS - 1 - zz;
 #pragma unroll
                     for (int k = 0; k < kN / 16; ++k)
                         mma_f16_ts(S::kLow && z ? d + D : d, p + (z ? 32 + 32 * z : 0) + k * 8, desc_of(vd + (k * 2048 >> 4)), kPvDesc,
-                                   k || z > (S::kLow ? 1 : 0) ? 1u : (fresh ? 0u : 1u));
+                                   k || zz > (S::kLow ? 1 : 0) ? 1u : ((S::kLow && z ? fresh_low : fresh) ? 0u : 1u));
+                }
                 tc_commit(o_done(t));
                 if (closes) tc_commit(o_last(t));
             };
@@ -767,8 +878,9 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                     if (alive && j < end) {
                         alive = hold(p_full(slot), p_phase >> buf & 1);
                         p_phase ^= 1u << buf;
+                        if (kT == 1 && alive && j > first && (j - first) % S::kSeg == 0) alive = hold(flushed, flushes++ & 1);
                         tc_fence_after();
-                        if (alive) weigh(slot, v_blk, j == first, j + 1 == end);
+                        if (alive) weigh(slot, v_blk, (j - first) % S::kSeg == 0, j == first, j + 1 == end);
                     }
                     free_block(v_blk);
                     if (alive && j + kBuf < last) {
@@ -806,21 +918,28 @@ __global__ void __launch_bounds__(TILES * 128) attn_join_kernel(const AttnArgs a
     if (rho >= (long long)jt.n * a.group) return;
     auto part = [&](int c) {
         const int slot = c == jt.c0 ? jt.slot0 : 2 * c;
-        return a.part + (size_t)(slot * TILES + t) * (D + 2) * kRowsTile + row;
+        return a.part + (size_t)(slot * TILES + t) * kPartFloats<D> + row * 4;
     };
     float m = -INFINITY;
-    for (int c = jt.c0; c <= jt.c1; ++c) m = fmaxf(m, __ldcg(part(c) + D * kRowsTile));
+    for (int c = jt.c0; c <= jt.c1; ++c) m = fmaxf(m, __ldcg(part_at(part(c), D)));
     float l = 0.0f, o[16];
 #pragma unroll
     for (int x = 0; x < 16; ++x) o[x] = 0.0f;
     for (int c = jt.c0; c <= jt.c1; ++c) {
-        const float *p = part(c);
-        const float mc = __ldcg(p + D * kRowsTile);
+        float *const p = part(c);
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_at(p, D)));
+        const float mc = ml.x;
         if (mc == -INFINITY) continue;                 // no key of this part is seen by the row
         const float f = exp2_approx(mc - m);
-        l = fmaf(__ldcg(p + (D + 1) * kRowsTile), f, l);
+        l = fmaf(ml.y, f, l);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) o[x] = fmaf(__ldcg(p + (size_t)(d0 + x) * kRowsTile), f, o[x]);
+        for (int x = 0; x < 16; x += 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_at(p, d0 + x)));
+            o[x] = fmaf(v.x, f, o[x]);
+            o[x + 1] = fmaf(v.y, f, o[x + 1]);
+            o[x + 2] = fmaf(v.z, f, o[x + 2]);
+            o[x + 3] = fmaf(v.w, f, o[x + 3]);
+        }
     }
     const float f = l > 0.0f ? __fdiv_rn(a.kv.v_scale, l) : (l == l ? 0.0f : l);
     const int tok = (int)(rho / a.group), h = jt.g * a.group + (int)(rho % a.group);
@@ -844,7 +963,7 @@ void launch(const AttnArgs &a, int sms, const CUtensorMap &k_map, const CUtensor
         TQ_CHECK(cudaFuncSetAttribute(attn_tile_kernel<D, LOAD, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
         set = true;
     }
-    JoinTile *joins = reinterpret_cast<JoinTile *>(a.part + (size_t)2 * sms * S::kTiles * (D + 2) * kRowsTile);
+    JoinTile *joins = reinterpret_cast<JoinTile *>(a.part + (size_t)2 * sms * S::kTiles * kPartFloats<D>);
     launch_pdl(attn_tile_kernel<D, LOAD, TERMS>, dim3(sms), dim3(S::kThreads), (size_t)S::kSmem, a, joins, k_map, v_map);
     TQ_LAUNCH_CHECK("attn_tile_kernel");
     launch_pdl(attn_join_kernel<D, S::kTiles, TERMS == 1>, dim3(sms, D / 16), dim3(S::kTiles * 128), 0, a, (const JoinTile *)joins);
@@ -871,8 +990,8 @@ void launch_dim(AttnArgs a, bool e4m3, int sms) {
 }  // namespace
 
 size_t attn_tile_part_floats(int sms) {
-    // two parts per CTA of 256 rows x (128 + 2), or 128 x (256 + 2), and the join kernel's list
-    return (size_t)2 * sms * 2 * (128 + 2) * kRowsTile + (size_t)sms * sizeof(JoinTile) / sizeof(float);
+    // two parts per CTA of two row tiles at dim 128, or of one at 256, and the join kernel's list
+    return (size_t)2 * sms * 2 * kPartFloats<128> + (size_t)sms * sizeof(JoinTile) / sizeof(float);
 }
 
 void launch_attn_tile(const AttnArgs &a, bool e4m3, int sms) {
