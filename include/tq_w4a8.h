@@ -450,8 +450,9 @@ int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, cons
 /* Attention of the new tokens over each request's cache: head h of a token at position p reads key/value head
  * h / (q_heads / heads) at positions 0..p, softmax(scale q.k) v. d_q: bf16 [tokens][q_heads][dim]. d_out: rows
  * [tokens][ldo] of q_heads * dim values, fp32 (computed to fp32's precision throughout; sums over keys lose 2^-17 of
- * the values' size at most, whatever the length) or, with out_bf16, bf16
- * (probabilities rounded to bf16 on the way). The cache behind d_kv_len[r] and unused pages are never read into a
+ * the values' size at most, whatever the length; over an e4m3 cache a probability carries 22 bits, none below 2^-36 of
+ * the row's largest) or, with out_bf16, bf16 (probabilities rounded to bf16 on the way, to fp16 over an e4m3 cache, and
+ * a quarter of a chunk's exponentials good to 2^-13.7). The cache behind d_kv_len[r] and unused pages are never read into a
  * result, whatever they hold; a value that is not finite below d_kv_len[r] may reach all rows of request r.
  * Returns as x_kv_append; the workspace that the first call makes is 40 MB whatever the sizes. */
 int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const uint16_t *d_q, int q_heads,

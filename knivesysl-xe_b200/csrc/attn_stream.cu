@@ -25,7 +25,10 @@
 // cache: e4m3 is exact in fp16, and a query row times a power of two that brings its largest value
 // to [2^9, 2^10) loses only what lies 2^-34 below that). Probabilities enter the second product as
 // one bf16 term for bf16 outputs (fp16 with an e4m3 cache), and for fp32 outputs as three bf16 terms
-// or two fp16 ones, 24 and 22 bits. All sums are fp32; for fp32 outputs they leave the tensor core, which
+// or two fp16 ones, 24 and 22 bits. fp16 ends at 2^-24, so its probabilities are taken 2^15 times as large
+// (2^11 in attn_tile.cu), above and below the fraction line: what is lost of one is 2^-40 (2^-36) of the
+// row's largest. Without that a key that outweighs the others by 2^16 takes digits from their sum, and one by
+// 2^25 all of it. All sums are fp32; for fp32 outputs they leave the tensor core, which
 // cuts them off, after every block of 16 keys.
 #include "attn.cuh"
 
@@ -40,6 +43,7 @@ constexpr int kW = 4;                 // warps of a CTA
 constexpr int kKeys = 16;             // keys of a warp's block
 constexpr int kUnit = kW * kKeys;     // keys of a unit
 constexpr int kRows = 16;             // query rows of a tile
+constexpr float kLift = 15.0f;        // of the exponents of fp16 probabilities: the largest is 2^15
 
 template <int D, bool E4M3>
 struct Shape {
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(kW * 32, (Shape<D, E4M3>::kCtas)) attn_stream_
                         o[t][2 * h + 1] *= f;
                     }
                 }
-                const float base = top[h] == -INFINITY ? 0.0f : top[h];
+                const float base = (top[h] == -INFINITY ? 0.0f : top[h]) - (E4M3 ? kLift : 0.0f);
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll

@@ -18,7 +18,9 @@
 //            products of two tiles takes one thread longer (2060 clocks per 64 keys at dim 128) than the
 //            tensor core needs for them (1310)
 // O is rescaled only when a row's maximum grows by more than 2^8: until then probabilities are up to
-// 2^8 instead of 1, which costs no precision, and the rescaling pass over O hardly ever runs.
+// 2^8 instead of 1, which costs no precision, and the rescaling pass over O hardly ever runs. fp16
+// probabilities (e4m3 cache) are 2^11 times as large, for fp16's range, and there it is 2^4 (2^14 and 2^1: the
+// chunks that kSeg's comment times take 246 us over an e4m3 cache of dim 128, instead of 218).
 //
 // What bounds it. bf16 outputs: the products of two tiles and 64 keys take 1024 clocks at dim 128, their
 // 16384 exponentials as long on the special-function units, next to maxima, sums and packing on the same
@@ -191,7 +193,7 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
     return d;
 }
-// 2^x for a pair, x <= 8, by the FMA pipe: x = n + f with |f| <= 1/2 (n rounded off by adding 1.5 x 2^23),
+// 2^x for a pair, x <= 15, by the FMA pipe: x = n + f with |f| <= 1/2 (n rounded off by adding 1.5 x 2^23),
 // 2^f a cubic with the smallest relative error on that interval, 7.5e-5 (fitted by Remez exchange),
 // and n added to its exponent. x below -126 (-inf too: a masked key) gives 2^-126
 // or so, which is nothing beside the row's largest, 1.
@@ -244,6 +246,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
     constexpr bool E4M3 = LOAD == kRegsE4m3;
     constexpr int kT = S::kTiles, kN = S::kKeys;
     constexpr bool OUT_BF16 = TERMS == 1;
+    constexpr float kLift = E4M3 ? 11.0f : 0.0f, kLag = E4M3 ? 4.0f : 8.0f;    // of the probabilities' exponents, of the maximum's
     constexpr int kBuf = S::kBuf, kScores = kT * kBuf;
     constexpr uint32_t kSlotCol = 256;                 // tensor memory: O tiles (and the lower terms' sums), then the slots of S and P
     constexpr uint32_t kQkDesc = idesc_f16(128, kN, !E4M3, false), kPvDesc = idesc_f16(128, D, !E4M3, true);
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                                 before = s_m[row];
                             }
                         }
-                        const bool grows = mx > before + 8.0f;
+                        const bool grows = mx > before + kLag;
                         const float now = grows ? mx : before;
                         if constexpr (kGroups == 2) {
                             s_m[row] = now;
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                             l *= exp2_approx(m - now);
                             m = now;
                         }
-                        const float off = m == -INFINITY ? 0.0f : -m;
+                        const float off = m == -INFINITY ? 0.0f : kLift - m;
                         // ---- probabilities, over the scores
                         f32x2 sum = pack2(0.0f, 0.0f);
                         const f32x2 c2 = pack2(c, c), off2 = pack2(off, off);

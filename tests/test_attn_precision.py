@@ -41,6 +41,50 @@ def _shared(b, count):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("e4m3", [False, True], ids=["bf16_cache", "e4m3_cache"])
+@pytest.mark.parametrize("depth", [16, 20, 24])
+@pytest.mark.parametrize("new,dim", [(1, 64), (1, 128), (1, 256), (100, 64), (100, 128), (100, 256)])
+def test_one_key_far_above_the_rest(lib, new, dim, depth, e4m3, bf16):
+    """The first key has nearly all the weight and the value 0; 8191 others, some 2^-depth of it each, carry the result
+    with values of one sign. Many requests share the pages, so that a CTA takes all keys of one.
+
+    Relative to the output, fp32: a score of size depth (in base 2) has a factor of three roundings and is itself rounded
+    beside the maximum, 4 depth ln 2 roundings of 2^-24; the exponentials, 2^-22 above and below; the sums' steps (see
+    SUMS). Two fp16 terms of an e4m3 cache's probabilities lose 2^-40 of the largest weight, above 16 rows 2^-36: 2^depth
+    as much of one of these, whose random part may put it 2^-1 lower. bf16: a rounding of a probability, 2^-9
+    (fp16 for e4m3: 2^-12, or where it ends), averaged over thousands but taken whole here, the exponentials' 7.5e-5, a
+    sum of all 8192 keys in steps of 16, and the store's 2^-9."""
+    total = 8192 + new - 1
+    b = ref.Batch([(new, total)], 64, 1, dim, e4m3, seed=depth + dim)
+    g, unit = b.gen, 16.0 if e4m3 else 1.0               # pools hold k / k_scale
+    p = np.arange(total)
+    page, slot = torch.from_numpy(b.table[0, p // 64]).long(), p % 64
+    k0 = torch.randn(total, generator=g) * 0.25
+    k0[0] = 8.0
+    k = b.k.float()
+    k[page, 0, slot, 0] = k0 * unit
+    v = b.v.float().abs() * 0.25 + b.v.float().abs().amax() * 0.25
+    v[page[0], 0, slot[0]] = 0.0
+    b.k.copy_(k.to(b.dtype))
+    b.v.copy_(v.to(b.dtype))
+    count = 320 if new == 1 else 80
+    one = _shared(b, count)
+    b.upload()
+    q = torch.zeros(b.tokens, 2, dim)
+    q[..., 0] = 1.0
+    q = q.to(torch.bfloat16)
+    scale = float(np.float32(depth * np.log(2.0) / 8.0))
+    got = _run(lib, b, q, 2, scale, bf16).double().reshape(count, new, -1)
+    want = ref.attention(one, q[:new], 2, scale)
+    bound = SUMS + (2.8 * depth + 8) * 2.0 ** -24 + (2.0 ** (depth - (39 if new == 1 else 35)) if e4m3 else 0.0)
+    if bf16:
+        bound += 2.0 ** -8 + 2.0 ** -13.7 + 1024 * 2.0 ** -24
+    off = ((got - want) / want).abs().max().item()
+    assert off <= bound, (off, bound)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("e4m3", [False, True], ids=["bf16_cache", "e4m3_cache"])
 @pytest.mark.parametrize("new", [1, 20])
 @pytest.mark.parametrize("dim", [64, 128, 256])
