@@ -932,7 +932,7 @@ __global__ void __launch_bounds__(TILES * 128) attn_join_kernel(const AttnArgs a
         float *const p = part(c);
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_at(p, D)));
         const float mc = ml.x;
-        if (mc == -INFINITY) continue;                 // no key of this part is seen by the row
+        if (mc == -INFINITY && ml.y == ml.y) continue; // no key of this part is seen by the row (or only such as give NaN)
         const float f = exp2_approx(mc - m);
         l = fmaf(ml.y, f, l);
 #pragma unroll

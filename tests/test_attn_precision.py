@@ -194,3 +194,29 @@ def test_a_maximum_that_keeps_growing(lib, new, dim, growth, e4m3, bf16):
     bound = 2.0 ** -8 if bf16 else SUMS + 5.6 * growth * 2.0 ** -24
     off = (got - want).abs().max().item()
     assert off <= top * bound, (off / top, bound)
+
+
+def _nan_key(lib, new, dim, e4m3, bf16, at):
+    """A key of NaN at position `at` of the first request: rows that see it are NaN, the others keep their values."""
+    b = ref.Batch([(new, 128 + new), (2, 90)], 16, 1, dim, e4m3, seed=at)
+    q = torch.randn(b.tokens, 2, dim, generator=b.gen).to(torch.bfloat16)
+    clean = ref.attention(b, q, 2, dim ** -0.5)
+    k = b.k.float()
+    k[b.table[0, at // 16], 0, at % 16] = float("nan")
+    b.k.copy_(k.to(b.dtype))
+    b.upload()
+    got = _run(lib, b, q, 2, dim ** -0.5, bf16).double()
+    sees = torch.zeros(b.tokens, dtype=torch.bool)
+    sees[max(0, at - 128):new] = True
+    assert torch.isnan(got[sees]).all()
+    top = b.v.double().abs().max() * b.v_scale
+    assert ((got[~sees] - clean[~sees]).abs() <= top * (2.0 ** -8 if bf16 else 2.0 ** -17)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("e4m3", [False, True], ids=["bf16_cache", "e4m3_cache"])
+@pytest.mark.parametrize("new,dim", [(3, 128), (100, 64), (100, 128), (100, 256)])
+def test_a_part_that_sees_one_key_of_nan(lib, new, dim, e4m3, bf16):
+    """The first row's last block of keys is another CTA's part, in which the row sees the first key alone."""
+    _nan_key(lib, new, dim, e4m3, bf16, 128)
