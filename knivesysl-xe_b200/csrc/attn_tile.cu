@@ -195,7 +195,7 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 }
 // 2^x for a pair, x <= 15, by the FMA pipe: x = n + f with |f| <= 1/2 (n rounded off by adding 1.5 x 2^23),
 // 2^f a cubic with the smallest relative error on that interval, 7.5e-5 (fitted by Remez exchange),
-// and n added to its exponent. x below -126 (-inf too: a masked key) gives 2^-126
+// times 2^n (a product, not an addition to the exponent: a NaN stays one). x below -126 (-inf too: a masked key) gives 2^-126
 // or so, which is nothing beside the row's largest, 1.
 __device__ __forceinline__ void exp2_cubic(f32x2 x, float &e0, float &e1) {
     float x0, x1, r0, r1;
@@ -204,14 +204,12 @@ __device__ __forceinline__ void exp2_cubic(f32x2 x, float &e0, float &e1) {
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
     x = pack2(x0, x1);
     const f32x2 r = add2(x, pack2(kMagicF, kMagicF));
-    const f32x2 f = add2(x, mul2(add2(r, pack2(-kMagicF, -kMagicF)), pack2(-1.0f, -1.0f)));
+    const f32x2 f = fma2(add2(r, pack2(-kMagicF, -kMagicF)), pack2(-1.0f, -1.0f), x);
     f32x2 p = fma2(pack2(0.0551716691f, 0.0551716691f), f, pack2(0.242611122f, 0.242611122f));
     p = fma2(p, f, pack2(0.693260985f, 0.693260985f));
     p = fma2(p, f, pack2(0.999928074f, 0.999928074f));
-    unpack2(p, e0, e1);
     unpack2(r, r0, r1);
-    e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(r0) << 23));
-    e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(r1) << 23));
+    unpack2(mul2(p, pack2(__uint_as_float((__float_as_uint(r0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(r1) << 23) + 0x3f800000u))), e0, e1);
 }
 
 // A wait of this kernel, by a whole warp: bounded, and given up at once when another wait of the CTA was.

@@ -220,3 +220,12 @@ def _nan_key(lib, new, dim, e4m3, bf16, at):
 def test_a_part_that_sees_one_key_of_nan(lib, new, dim, e4m3, bf16):
     """The first row's last block of keys is another CTA's part, in which the row sees the first key alone."""
     _nan_key(lib, new, dim, e4m3, bf16, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True], ids=["bf16_cache", "e4m3_cache"])
+@pytest.mark.parametrize("at", [1, 70, 71, 102, 133, 134, 135])
+def test_a_key_of_nan_at_any_place_of_a_block(lib, at, e4m3):
+    """bf16 outputs of chunks take some of a block's exponentials another way: those have to keep NaN too."""
+    for dim in (64, 128, 256):
+        _nan_key(lib, 100, dim, e4m3, True, at)
