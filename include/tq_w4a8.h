@@ -461,8 +461,8 @@ int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, con
  * bases[i][t]); up to 4 projections of one input, with the same K and number of adapters. x fp32 [T][K], bases and
  * ys fp32 [T][M]; bases[i] may be ys[i] (added in place) or NULL, as may bases (0). Products and sums are fp32's; an
  * infinity in x makes its row NaN.
- * No output may be x, another output or another projection's base (-2). M is at most 2^21 and count * M below 2^31
- * (-3). An adapter number beyond the pool or a rank out of range counts as none and leaves 10043 in tq_last_error().
+ * No output may overlap x, another output or another projection's base, nor its own base in part (-2). M is at most
+ * 2^21 and count * M below 2^31 (-3). An adapter number beyond the pool or a rank out of range counts as none and leaves 10043 in tq_last_error().
  * The scratch grows with T (up to 4096) and the ranks; what a captured graph uses stays. Returns as x_kv_append. */
 int qwn_x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *const *ys, int count,
                    const float *d_x, const int32_t *d_adapter, int T);

@@ -30,6 +30,10 @@ int kv_args(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, KvArgs &a);
 // A bf16 matrix of rows of `cols` values (a multiple of 8, 16-byte aligned), for TMA copies of box_rows rows x 64
 // values with the 128-byte swizzle, zeros outside; false if the driver refuses it.
 bool tensor_map_2d(CUtensorMap &map, const void *data, int cols, long long rows, int box_rows);
+// Whether the memory of two operands has bytes in common.
+inline bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 #ifdef __CUDACC__

@@ -674,11 +674,14 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
         a.y[i] = ys[i];
         if (!aligned16(ys[i]) || (a.base[i] && !aligned16(a.base[i]))) return -4;
     }
-    // an output is nobody else's, and x is read for all projections
+    // an output is nobody else's, and x is read for all projections; its own base is the output or apart from it
+    const auto bytes = [&](int cols) { return (size_t)T * cols * sizeof(float); };
     for (int i = 0; i < count; ++i) {
-        if (ys[i] == d_x) return -2;
+        const size_t mine = bytes(a.M[i]);
+        if (overlap(ys[i], mine, d_x, bytes(ws[0]->K))) return -2;
+        if (ys[i] != a.base[i] && overlap(ys[i], mine, a.base[i], mine)) return -2;
         for (int j = 0; j < count; ++j)
-            if (j != i && (ys[i] == ys[j] || ys[i] == a.base[j])) return -2;
+            if (j != i && (overlap(ys[i], mine, ys[j], bytes(a.M[j])) || overlap(ys[i], mine, a.base[j], bytes(a.M[j])))) return -2;
     }
     a.count = count;
     a.adapters = ws[0]->count;

@@ -308,3 +308,23 @@ def test_lora_refuses_bad_arguments(pkg):
     assert lib.qwn_x_lora_add(ws, None, one, 1, 4096, 4096, 4) == -2
     wide = pkg.lora_array([pkg.Lora(**(rec | dict(count=2048, M=1 << 20)))])
     assert lib.qwn_x_lora_add(wide, None, (C.c_void_p * 1)(8192), 1, 4096, 4096, 4) == -3
+
+
+def test_lora_refuses_outputs_that_overlap(pkg):
+    """In part, as much as by the same address: T = 4 rows of 64 values are 1024 bytes."""
+    lib = pkg.load()
+    rec = pkg.Lora(2, 16, 64, 64, 4096, 4096, None, None)
+    two = pkg.lora_array([rec, rec])
+    x = 1 << 20
+    ptrs = lambda *p: (C.c_void_p * len(p))(*p)  # noqa: E731
+
+    def call(ys, bases=None, n=1):
+        return lib.qwn_x_lora_add(two, ptrs(*bases) if bases else None, ptrs(*ys), n, x, 4096, 4)
+
+    for y in (x - 1008, x, x + 16, x + 1008):
+        assert call([y]) == -2, y
+    for base in (8192 - 1008, 8192 + 256):                       # rows of the base that other rows' results overwrite
+        assert call([8192], [base]) == -2, base
+    for y in (8192 - 1008, 8192 + 512):
+        assert call([8192, y], n=2) == -2, y
+        assert call([8192, 65536], [None, y], n=2) == -2, y
