@@ -523,6 +523,10 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     // packed rows (new tokens x group) are counted in 32 bits
     if ((long long)a.kv.tokens * q_heads > 0x7fffff00ll) return -3;
     if (!aligned16(d_q) || !aligned16(d_out) || ldo % (out_bf16 ? 8 : 4)) return -4;
+    // A tile's rows are written after all that read its queries have done so: in place the two may be the same rows
+    const size_t width = (size_t)q_heads * D, q_bytes = a.kv.tokens * width * 2;
+    const size_t out_bytes = ((a.kv.tokens - 1) * ldo + width) * (out_bf16 ? 2 : 4);
+    if (overlap(d_out, out_bytes, d_q, q_bytes) && !(d_out == d_q && out_bf16 && ldo == width)) return -2;
     if (const int rc = attn_scratch(sm_count())) return rc;
     if (!device_status_ready()) return -40;
     a.kv.status = device_status_word();

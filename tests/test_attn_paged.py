@@ -213,3 +213,33 @@ def test_attention_refuses_bad_arguments(pkg):
         a = good | change
         assert lib.qwn_x_attn_paged(C.byref(cache), C.byref(batch), a["q"], a["heads"], a["scale"], a["out"], a["ldo"],
                                     a["bf16"]) == rc, change
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("lens", [[(1, 900), (1, 30), (1, 2500), (1, 64)], [(300, 900), (1, 2000), (70, 70)]], ids=["decode", "chunks"])
+def test_attention_in_place_of_the_queries(lib, lens, e4m3):
+    """bf16 rows over the queries themselves: the bits of the call with an output of its own, tiles cut or not."""
+    b = ref.Batch(lens, 16, 2, 128, e4m3, seed=31).upload()
+    q = torch.randn(b.tokens, 10, 128, generator=b.gen).to(torch.bfloat16)
+    want = _run(lib, b, q, 5, 0.1, True)
+    for _ in range(3):
+        dq = ref.up(q)
+        assert lib.qwn_x_attn_paged(C.byref(b.cache), C.byref(b.batch), dq.ptr, 10, 0.1, dq.ptr, 1280, 1) == 0
+        lib.tq_sync()
+        assert np.array_equal(ref.bits(ref.down(dq, torch.bfloat16, want.shape)), ref.bits(want))
+
+
+def test_attention_refuses_an_output_over_its_queries(pkg):
+    """4 tokens x 2 heads x 64 values are 1024 bytes of queries."""
+    lib = pkg.load()
+    cache = pkg.KvCache(4096, 4096, 4, 16, 2, 64, 0, 1.0, 1.0)
+    batch = pkg.KvBatch(1, 4, 4, 4, 4096, 4096, 4096)
+    q = 1 << 20
+
+    def call(out, ldo, bf16):
+        return lib.qwn_x_attn_paged(C.byref(cache), C.byref(batch), q, 2, 0.125, out, ldo, bf16)
+
+    for out, ldo, bf16 in [(q, 128, 0), (q, 136, 1), (q + 16, 128, 1), (q - 1008, 128, 1), (q - 2032, 128, 0), (q + 1008, 128, 1),
+                           (q - 2 * (3 * 256 + 128) + 16, 256, 1)]:
+        assert call(out, ldo, bf16) == -2, (out - q, ldo, bf16)
