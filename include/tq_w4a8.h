@@ -441,7 +441,8 @@ typedef struct {
  * to the cache, rounded once. d_q, d_k, d_v: fp32 rows of the projections, ldq / ldk / ldv values apart (so they may
  * be columns of one wide matrix); all 16-byte aligned, the strides multiples of 4. q_heads = 0 with d_q and d_q_out
  * NULL: keys and values only. rope NULL: neither norm nor rotation. e4m3 values beyond +-448 scales become +-448.
- * Two requests that share a page must not both write to it in one call.
+ * Two requests that share a page must not both write to it in one call, nor may a request's new tokens find one page
+ * twice in its table. d_q_out must not lie among the rows of d_q, d_k or d_v (-2).
  * Returns 0, -1 (bad record), -2 (bad arguments), -3 (sizes outside the kernels' range), -4 (alignment), -40 (the
  * process's first call that needs device memory of the library's own, made while the stream is being captured). */
 int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq_rope_t *rope, const float *d_q,

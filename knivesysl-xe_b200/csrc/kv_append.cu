@@ -291,6 +291,12 @@ int x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq
     if ((q_heads && (!aligned16(d_q) || !aligned16(d_q_out) || ldq % 4)) || !aligned16(d_k) || !aligned16(d_v) || ldk % 4 ||
         ldv % 4)
         return -4;
+    // the queries' rows are stored while other rows are being read
+    const auto span = [&](size_t ld, int heads) { return ((a.kv.tokens - 1) * ld + (size_t)heads * D) * sizeof(float); };
+    const size_t out_bytes = (size_t)a.kv.tokens * q_heads * D * sizeof(uint16_t);
+    if (overlap(d_q_out, out_bytes, d_q, span(ldq, q_heads)) || overlap(d_q_out, out_bytes, d_k, span(ldk, a.kv.heads)) ||
+        overlap(d_q_out, out_bytes, d_v, span(ldv, a.kv.heads)))
+        return -2;
     if (!device_status_ready()) return -40;
     a.kv.status = device_status_word();
     a.q = d_q;

@@ -188,3 +188,12 @@ def test_append_refuses_bad_arguments(pkg):
     cache, batch = _fake(pkg, batch_tokens=0)
     assert lib.qwn_x_kv_append(C.byref(cache), C.byref(batch), None, None, 0, 0, None, 4096, 128, 4096, 128) == 0
     assert lib.qwn_x_attn_paged(C.byref(cache), C.byref(batch), 4096, 2, 0.125, 4096, 128, 0) == 0
+
+
+def test_append_refuses_queries_out_over_its_inputs(pkg):
+    """One token, 2 heads of 64: 256 bytes of queries out, 512 of q rows and 512 of k and of v rows."""
+    lib = pkg.load()
+    cache, batch = _fake(pkg)
+    q, k, v = 1 << 20, 2 << 20, 3 << 20
+    for out in (q, q + 496, q - 240, k, k + 256, v - 240, v + 496):
+        assert lib.qwn_x_kv_append(C.byref(cache), C.byref(batch), None, q, 128, 2, out, k, 128, v, 128) == -2, out
