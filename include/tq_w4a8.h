@@ -455,7 +455,7 @@ int qwn_x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, cons
  * the row's largest) or, with out_bf16, bf16 (probabilities rounded to bf16 on the way, to fp16 over an e4m3 cache, and
  * a quarter of a chunk's exponentials good to 2^-13.7). The cache behind d_kv_len[r] and unused pages are never read into a
  * result, whatever they hold; a value that is not finite below d_kv_len[r] may reach all rows of request r.
- * d_out may be d_q with bf16 rows of the same stride, and not overlap it otherwise (-2).
+ * scale is finite, in base 2 and times k_scale too (-2). d_out may be d_q with bf16 rows of the same stride, and not overlap it otherwise (-2).
  * Returns as x_kv_append; the workspace that the first call makes is 40 MB whatever the sizes. */
 int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const uint16_t *d_q, int q_heads,
                      float scale, void *d_out, size_t ldo, int out_bf16);

@@ -517,6 +517,8 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     if (const int rc = kv_args(cache, batch, a.kv)) return rc;
     const int D = a.kv.dim;
     if (q_heads <= 0 || !(fabsf(scale) < INFINITY) || (out_bf16 != 0 && out_bf16 != 1)) return -2;
+    a.c = scale * a.kv.k_scale * 1.4426950408889634f;
+    if (!(fabsf(a.c) < INFINITY)) return -2;
     if (q_heads % a.kv.heads || q_heads > 65535) return -3;
     if (!a.kv.count || !a.kv.tokens || !a.kv.max_new) return 0;
     if (!d_q || !d_out || ldo < (size_t)q_heads * D) return -2;
@@ -535,7 +537,6 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     a.ldo = ldo;
     a.q_heads = q_heads;
     a.group = q_heads / a.kv.heads;
-    a.c = scale * a.kv.k_scale * 1.4426950408889634f;
     a.out_bf16 = out_bf16;
     a.part = g_attn.part;
     a.arrived = g_attn.arrived;

@@ -243,3 +243,12 @@ def test_attention_refuses_an_output_over_its_queries(pkg):
     for out, ldo, bf16 in [(q, 128, 0), (q, 136, 1), (q + 16, 128, 1), (q - 1008, 128, 1), (q - 2032, 128, 0), (q + 1008, 128, 1),
                            (q - 2 * (3 * 256 + 128) + 16, 256, 1)]:
         assert call(out, ldo, bf16) == -2, (out - q, ldo, bf16)
+
+
+def test_attention_refuses_a_scale_that_overflows(pkg):
+    """The scale goes by the cache's and into base 2 in fp32."""
+    lib = pkg.load()
+    batch = pkg.KvBatch(1, 1, 1, 4, 4096, 4096, 4096)
+    for k_scale, e4m3, scale in [(2.0 ** 100, 1, 2.0 ** 100), (1.0, 0, 3e38), (1.0, 0, -3e38)]:
+        cache = pkg.KvCache(4096, 4096, 4, 16, 2, 64, e4m3, k_scale, 1.0)
+        assert lib.qwn_x_attn_paged(C.byref(cache), C.byref(batch), 8192, 2, scale, 4096, 128, 0) == -2, (k_scale, scale)
