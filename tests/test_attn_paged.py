@@ -252,3 +252,29 @@ def test_attention_refuses_a_scale_that_overflows(pkg):
     for k_scale, e4m3, scale in [(2.0 ** 100, 1, 2.0 ** 100), (1.0, 0, 3e38), (1.0, 0, -3e38)]:
         cache = pkg.KvCache(4096, 4096, 4, 16, 2, 64, e4m3, k_scale, 1.0)
         assert lib.qwn_x_attn_paged(C.byref(cache), C.byref(batch), 8192, 2, scale, 4096, 128, 0) == -2, (k_scale, scale)
+
+
+def _many(count, longest, seed):
+    """Requests of one token, one in five without any, lengths over the whole range."""
+    g = np.random.default_rng(seed)
+    return [(int(i % 5 != 3), int(g.integers(1, longest))) for i in range(count)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # more requests than the decode kernel has threads, across one and several blocks of them
+    (_many(129, 60, 1), 16, 2, 4, 64, False),
+    (_many(300, 200, 2), 16, 1, 8, 128, True),
+    (_many(700, 40, 3), 7, 2, 1, 256, False),
+    ([(0, 5)] * 256 + [(1, 90)] + [(0, 0)] * 200 + [(1, 7)], 16, 2, 2, 64, False),
+    # and than the kernel for chunks has
+    (_many(460, 60, 4) + [(150, 300)] + _many(50, 90, 5), 16, 2, 2, 128, False),
+    (_many(500, 40, 6) + [(40, 40)], 20, 1, 6, 64, False),
+    ([(30, 45)] + _many(470, 40, 7) + [(90, 333)], 16, 1, 2, 256, True),
+    # a request of more row tiles than that has threads
+    ([(3, 9), (700, 700), (1, 40)], 64, 1, 64, 64, False),
+], ids=[str(i) for i in range(8)])
+def test_attention_of_more_requests_and_tiles_than_threads(lib, case):
+    lens, page, heads, group, dim, e4m3 = case
+    for bf16 in (False, True):
+        _check(lib, ref.Batch(lens, page, heads, dim, e4m3, seed=len(lens)), group, bf16)
