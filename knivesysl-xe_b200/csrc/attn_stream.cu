@@ -484,12 +484,6 @@ int attn_scratch(int sms) {
     return 0;
 }
 
-int sm_count() {
-    static int n = 0;
-    if (!n) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, tq_device());
-    return n > 0 ? n : 148;
-}
-
 template <int D, bool E4M3, bool OUT_BF16>
 void launch_stream(const AttnArgs &a) {
     using S = Shape<D, E4M3>;
@@ -498,7 +492,7 @@ void launch_stream(const AttnArgs &a) {
         TQ_CHECK(cudaFuncSetAttribute(attn_stream_kernel<D, E4M3, OUT_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
         set = true;
     }
-    launch_pdl(attn_stream_kernel<D, E4M3, OUT_BF16>, dim3(sm_count() * S::kCtas), dim3(kW * 32), (size_t)S::kSmem, a);
+    launch_pdl(attn_stream_kernel<D, E4M3, OUT_BF16>, dim3(gpu_sms() * S::kCtas), dim3(kW * 32), (size_t)S::kSmem, a);
     TQ_LAUNCH_CHECK("attn_stream_kernel");
 }
 template <int D>
@@ -529,7 +523,7 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     const size_t width = (size_t)q_heads * D, q_bytes = a.kv.tokens * width * 2;
     const size_t out_bytes = ((a.kv.tokens - 1) * ldo + width) * (out_bf16 ? 2 : 4);
     if (overlap(d_out, out_bytes, d_q, q_bytes) && !(d_out == d_q && out_bf16 && ldo == width)) return -2;
-    if (const int rc = attn_scratch(sm_count())) return rc;
+    if (const int rc = attn_scratch(gpu_sms())) return rc;
     if (!device_status_ready()) return -40;
     a.kv.status = device_status_word();
     a.q = d_q;
@@ -543,7 +537,7 @@ int x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const u
     a.limit_ns = wait_limit_ns();
     const bool e4m3 = cache->e4m3 != 0;
     if ((long long)a.kv.max_new * a.group > kRows) {
-        launch_attn_tile(a, e4m3, sm_count());
+        launch_attn_tile(a, e4m3, gpu_sms());
         return 0;
     }
     if (D == 64) launch_stream<64>(a, e4m3);

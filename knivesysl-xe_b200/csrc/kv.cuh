@@ -16,6 +16,7 @@ constexpr int kStatusAdapter = 43;   // an adapter number or rank out of range (
 
 // Whether scratch may be allocated now: not while the stream is captured into a graph.
 bool stream_is_capturing();
+int gpu_sms();                       // SMs of the device
 
 struct KvArgs {
     uint8_t *k, *v;              // [pages][heads][page_size][dim]

@@ -217,6 +217,12 @@ bool stream_is_capturing() {
     return cudaStreamIsCapturing(stream(), &st) != cudaSuccess || st != cudaStreamCaptureStatusNone;
 }
 
+int gpu_sms() {
+    static int n = 0;
+    if (!n) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, tq_device());
+    return n > 0 ? n : 148;
+}
+
 bool tensor_map_2d(CUtensorMap &map, const void *data, int cols, long long rows, int box_rows) {
     static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         void *f = nullptr;
@@ -310,7 +316,7 @@ int x_kv_append(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, const tq
     const int rows = q_heads + 2 * a.kv.heads;
     // As few warps a token as fill the GPU (32 an SM): the request, its page and the angles are looked up once a warp,
     // which costs as much as some ten head rows. 2156 tokens of 56 rows: 28 us with 8 warps a token.
-    const long long want = 32ll * 148;
+    const long long want = 32ll * gpu_sms();
     a.parts = (int)std::min<long long>(rows, (want + a.kv.tokens - 1) / a.kv.tokens);
     a.rows_per_warp = (rows + a.parts - 1) / a.parts;
     const long long warps = (long long)a.kv.tokens * a.parts;

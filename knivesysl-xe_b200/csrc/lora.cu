@@ -635,12 +635,6 @@ __global__ void __launch_bounds__(kThreadsE, 1)
 float *g_h = nullptr;
 size_t g_h_floats = 0;
 
-int sm_count() {
-    static int n = 0;
-    if (!n) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, tq_device());
-    return n > 0 ? n : 148;
-}
-
 }  // namespace
 }  // namespace tq
 
@@ -689,7 +683,7 @@ int x_lora_add(const tq_lora_t *const *ws, const float *const *bases, float *con
     a.T = T;
     a.x = d_x;
     a.adapter = d_adapter;
-    const int sms = sm_count();
+    const int sms = gpu_sms();
     // a call of more tokens than a CTA sorts goes in pieces
     const int piece = std::min(T, kMaxTokens), k64 = (a.K + 63) / 64;
     const int tiles = (piece + kTok - 1) / kTok + std::min(piece, a.adapters);     // at most
