@@ -69,7 +69,7 @@ struct TileShape {
     // to 2^-23 of it, twice in a step of 16 keys: n cuts of a sum that grows evenly take n 2^-24. fp32 outputs: 128 cuts at
     // most, and 4e-6 was the most measured; without it 35000 keys in a row lose 1.5e-4 (two terms), 1.8e-4 (lower terms
     // apart) or 4e-4 (three terms in one sum). bf16 outputs: 140000 keys lost 8e-4 of themselves. Chunks of 1024 and 512
-    // tokens on 3000 and 1500, fp32: 189 -> 203 us at dim 128, 126 -> 134 at 64, 197 -> 258 at 256, where a sum of all
+    // tokens on 3000 and 1500, fp32: 189 -> 203 us at dim 128, 126 -> 134 at 64, 197 -> 249 at 256, where a sum of all
     // three terms has to leave every 256 keys.
     static constexpr int kSeg = TERMS == 1 ? 128 : (kLow ? 16 : (TERMS == 2 ? 8 : 4));
     static constexpr int kBlock = kKeys * D * 2;                    // bytes of keys, or of values
@@ -157,9 +157,9 @@ __device__ __forceinline__ float4 ld_sums(const float *p) {
 // COLS dims of a row's sums leave tensor memory for those in global memory (the tile's place among the parts, whether or
 // not it is cut): stored the first time (`once`), then added. Adding without reading has nothing to wait for; one thread's
 // additions to an address keep their order. The sums outside go by the maximum *ref, those in tensor memory by `top`, which
-// is no smaller; grown by more than 2^8, it scales the former first. Out of line: the block loop has no registers to spare.
+// is no smaller; grown by more than 2^8, it scales the former first.
 template <int COLS>
-static __device__ __noinline__ void flush_sums(float *part, uint32_t o_col, float *ref_at, bool once, float top) {
+__device__ __forceinline__ void flush_sums(float *part, uint32_t o_col, float *ref_at, bool once, float top) {
     float ref = once ? top : *ref_at;
     if (__any_sync(0xffffffffu, top > ref + 8.0f)) {
         const float by = top == -INFINITY ? 1.0f : exp2_approx(ref - top);
@@ -186,6 +186,14 @@ static __device__ __noinline__ void flush_sums(float *part, uint32_t o_col, floa
             else add_sums(part_at(part, x + y), z);
         }
     }
+}
+
+// The same out of line, where the block loop has no registers to spare: a call costs the loop some as well. Measured, inline
+// and called: 2048 new tokens, dim 128, bf16 in and out 87 and 98 us; the chunks of kSeg's times at dim 256, fp32 249 and 258,
+// bf16 162 and 156, dim 128 over e4m3, bf16, 166 and 156; else within 1 %.
+template <int COLS>
+static __device__ __noinline__ void flush_sums_call(float *part, uint32_t o_col, float *ref_at, bool once, float top) {
+    flush_sums<COLS>(part, o_col, ref_at, once, top);
 }
 
 __device__ __forceinline__ float max3(float x, float y, float z) {
@@ -433,7 +441,10 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
             float m = -INFINITY, l = 0.0f, c_next = 0.0f;
             // This warpgroup's share of O, which has the maximum `top`, leaves for sums outside (see flush_sums).
             auto flush = [&](bool once, float top) {
-                flush_sums<D / kGroups>(part_at(cur.part, wg * (D / kGroups)), o_col + wg * (D / kGroups), s_ref + tid, once, top);
+                float *const part = part_at(cur.part, wg * (D / kGroups));
+                const uint32_t col = o_col + wg * (D / kGroups);
+                if constexpr (LOAD == kTma && (D <= 128 || TERMS > 1)) flush_sums<D / kGroups>(part, col, s_ref + tid, once, top);
+                else flush_sums_call<D / kGroups>(part, col, s_ref + tid, once, top);
             };
             Part next = cur;
             next.last = next.first;                        // none
