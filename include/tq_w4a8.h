@@ -403,11 +403,13 @@ typedef struct {
  * d_start[r + 1] - 1, and d_kv_len[r] tokens in the cache INCLUDING them: its new tokens stand at the positions
  * d_kv_len[r] - new .. d_kv_len[r] - 1. Position p lies in slot p % page_size of page d_pages[r * max_pages +
  * p / page_size]. A request may have no new token. tokens: rows of the matrices (those from d_start[count] on are
- * padding and left alone); max_new: no request has more new tokens (bounds what is launched). The three arrays are
- * device memory, read when the kernels run. What is impossible in them (ranges that fall or leave the matrix,
- * more new tokens than cached ones, more than max_pages pages, a page outside the pool) is found there: the request
- * is skipped (a bad page's slots: not written, and read as zeros) and tq_last_error() gives 10041 after tq_sync(), or 10042 for more new tokens
- * than max_new. */
+ * padding and left alone); max_new: no request has more new tokens (0: there is nothing to do, and nothing is looked
+ * at). It chooses the attention's kernel for the whole batch: up to 16 rows (max_new x query heads a key/value head)
+ * the one that reads the cache at the memory's rate, above it one for chunks, in which a decode batch takes 2.3 to 2.8
+ * times as long. The three arrays are device memory, read when the kernels run. What is impossible in them (ranges
+ * that fall or leave the matrix, more new tokens than cached ones, more than max_pages pages, a page outside the pool)
+ * is found there: the request is skipped (a bad page's slots: not written, and read as zeros) and tq_last_error() gives
+ * 10041 after tq_sync(), or 10042 for more new tokens than max_new. */
 typedef struct {
     int count, tokens, max_new, max_pages;
     const int32_t *d_start;
@@ -462,7 +464,8 @@ int qwn_x_attn_paged(const tq_kv_cache_t *cache, const tq_kv_batch_t *batch, con
 /* ys[i][t] = bases[i][t] + scale (x[t] A^T) B^T with the adapter d_adapter[t] of ws[i] (negative: none, the row is
  * bases[i][t]); up to 4 projections of one input, with the same K and number of adapters. x fp32 [T][K], bases and
  * ys fp32 [T][M]; bases[i] may be ys[i] (added in place) or NULL, as may bases (0). Products and sums are fp32's; an
- * infinity in x makes its row NaN.
+ * infinity in x makes its row NaN. The same call gives the same bits, but a row's last bits depend on the batch that
+ * it is in: the order of the sums over K follows the tokens that share an adapter.
  * No output may overlap x, another output or another projection's base, nor its own base in part (-2). M is at most
  * 2^21 and count * M below 2^31 (-3). An adapter number beyond the pool or a rank out of range counts as none and leaves 10043 in tq_last_error().
  * The scratch grows with T (up to 4096) and the ranks; what a captured graph uses stays. Returns as x_kv_append. */

@@ -13,13 +13,15 @@
 // rings of their own (cp.async, no barrier between warps). A tile that several CTAs share is joined
 // by the last of them to finish, in the order of the keys, so results do not depend on timing.
 //
-// The rule: at most 16 packed rows a head. Decoding through the kernel of 128-row tiles instead takes 38 us
-// for one request, 159 us for 64 (here 13.5 and 65) and 187 us for 8 long e4m3 caches (here 73): its ring
-// and its barriers wait for 128 rows of products where 16 are wanted. Above 16 rows this one would read the
-// cache again for every 16. Measured: 64 requests, bf16, 336 MB of cache: 65 us, 5.2 TB/s; 8 long e4m3
-// caches of dim 256, 171 MB: 73 us, 2.3 TB/s, where turning e4m3 into fp16 (a conversion per two values at
-// a quarter rate) and the latency of two blocks in flight a warp weigh more than the bytes; one request:
-// 13.5 us, latency of launch, first bytes and join.
+// The rule: at most 16 packed rows a head, max_new x group, the same kernel for the whole batch. Decoding
+// through the kernel of 128-row tiles instead took 38 us for one request, 159 us for 64 and 187 us for 8
+// long e4m3 caches, where this one takes 14, 71 and 78: its ring and its barriers wait for 128 rows of
+// products where 16 are wanted. Above 16 rows this one would need a second row tile beside the first (not
+// built), or read the cache again for every 16. Measured: 64 requests, bf16, 336 MB of cache: 71 us,
+// 4.8 TB/s; 8 long e4m3 caches of dim 256, 171 MB: 78 us, 2.2 TB/s: six query rows in a tile of 16, so most
+// products and exponentials are for rows that do not exist, each warp waits on its own chain of conversion,
+// product and exponential, and 255 registers leave two warps a scheduler; one request: 13.7 us, latency
+// of launch, first bytes and join.
 //
 // Roundings: the products q.k are exact in the tensor core (bf16 x bf16, or fp16 x fp16 for an e4m3
 // cache: e4m3 is exact in fp16, and a query row times a power of two that brings its largest value

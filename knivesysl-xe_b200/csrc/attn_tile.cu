@@ -25,10 +25,11 @@
 // What bounds it. bf16 outputs: the products of two tiles and 64 keys take 1024 clocks at dim 128, their
 // 16384 exponentials as long on the special-function units, next to maxima, sums and packing on the same
 // four warps a tile: the softmax warpgroups set the pace. One pair of exponentials in four goes to the FMA
-// pipe. 4096 new tokens (32 query, 8 key/value heads of 128): 462 us = 0.67 of the measured bf16 rate by
-// operations (311 us). fp32 outputs carry P in three terms, four products instead of two: a batch of
-// chunks and decodes takes 273 us, 0.40 of the rate by the operations issued (110 us); there the split of P
-// into terms, 12 instructions a pair, takes longer than the products. One warpgroup a tile: 303 us.
+// pipe. 4096 new tokens on as many (40 query, 8 key/value heads of 128): 470 us in a run of that call alone = 0.66 of the
+// measured bf16 rate by operations (311 us). fp32 outputs carry P in three terms, four products instead of two: a
+// batch of chunks and decodes takes 278 us, 0.40 of the rate by the operations issued (110 us); there the split of P
+// into terms, 12 instructions a pair, takes longer than the products, and there is one row tile a CTA. With one
+// warpgroup a tile it took 30 us more.
 //
 // Work is cut into equal stretches of key blocks, one per SM (Line, kv.cuh): a causal batch of any
 // lengths loads all SMs alike. A tile cut between CTAs leaves (m, sum, O) of each part in global
@@ -49,7 +50,7 @@ namespace {
 constexpr int kRowsTile = 128;
 // How the load warps bring a block in.
 enum Load { kTma, kRegs, kRegsE4m3 };
-constexpr int kCubic = 1;             // of four pairs of exponentials, those that the FMA pipe computes (0, 1, 2, 3: 480, 462, 481, 522 us at 4096 tokens)
+constexpr int kCubic = 1;             // of four pairs of exponentials, those that the FMA pipe computes (0, 1, 2, 3: 480, 462, 481, 522 us at 4096 tokens, before the sums left tensor memory)
 
 template <int D, Load LOAD, int TERMS>
 struct TileShape {

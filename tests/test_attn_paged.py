@@ -278,3 +278,25 @@ def test_attention_of_more_requests_and_tiles_than_threads(lib, case):
     lens, page, heads, group, dim, e4m3 = case
     for bf16 in (False, True):
         _check(lib, ref.Batch(lens, page, heads, dim, e4m3, seed=len(lens)), group, bf16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True], ids=["bf16", "e4m3"])
+def test_attention_of_a_mixed_step_in_two_calls(lib, pkg, e4m3):
+    """Single tokens, then chunks: a record of each sort's requests over the same arrays. Rows of the other sort stay."""
+    lens = [(1, 700), (1, 3), (0, 90), (1, 1200), (60, 300), (0, 0), (150, 150)]
+    b = ref.Batch(lens, 16, 2, 128, e4m3, seed=77, pad=3).upload()
+    q = torch.randn(b.tokens, 10, 128, generator=b.gen).to(torch.bfloat16)
+    want = ref.attention(b, q, 5, 0.1)
+    dq, out = ref.up(q), ref.up(torch.full((b.tokens, 1280), 5.0))
+    cut, n = 4, len(lens)
+    for r0, r1, most in ((0, cut, 1), (cut, n, 150)):
+        part = pkg.KvBatch(r1 - r0, b.tokens, most, b.table.shape[1], b.dstart.ptr + 4 * r0, b.dlen.ptr + 4 * r0,
+                           b.dtable.ptr + 4 * r0 * b.table.shape[1])
+        assert lib.qwn_x_attn_paged(C.byref(b.cache), C.byref(part), dq.ptr, 10, 0.1, out.ptr, 1280, 0) == 0
+        lib.tq_sync()
+        assert lib.tq_last_error() == 0
+        got = ref.down(out, torch.float32, (b.tokens, 1280))
+        done = slice(0, b.start[r1])
+        assert (got[done].double() - want[done]).abs().max() <= b.v.double().abs().max() * b.v_scale * F32
+        assert (got[b.start[r1]:] == 5.0).all()
