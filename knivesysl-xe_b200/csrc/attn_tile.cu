@@ -564,7 +564,7 @@ __global__ void __launch_bounds__((TileShape<D, LOAD, TERMS>::kThreads), 1)
                         weights(v1, 32);
                         if (anew) {
                             // O holds the blocks up to j - 1 (the barrier is at most one phase behind, as above)
-                            if (!wait(o_done(t), (done - 1) & 1)) { alive = false; break; }
+                            if (!wait(o_done(t), (done - 1) & 1)) { tmem_wait_st(); alive = false; break; }
                             tc_fence_after();
                             flush(j - seg == S::kSeg, before);
                         }
